@@ -388,6 +388,86 @@ int sqattn_cache_append(void* k_cache, void* v_cache, const void* k_new, const v
                         int64_t cache_seq_stride, int64_t cache_row_stride, int64_t new_seq_stride, int32_t batch,
                         int32_t row_elems, int64_t capacity, sqattn_stream_t stream);
 
+/* ---- paged key/value cache (no counterpart in the reference, whose cache is one block per sequence) ----------- */
+
+enum {
+  SQATTN_KV_NATIVE = 0, /* 16-bit values */
+  SQATTN_KV_INT8 = 1,   /* int8 codes and one fp32 scale a row (token and KV head) */
+  SQATTN_KV_INT4 = 2    /* 4-bit codes, two to a byte (even channel in the low half), and one fp32 scale a row */
+};
+
+/* One layer's pages, all contiguous: k_pages, v_pages [num_pages, num_kv_heads, page_size, row], a row being head_dim
+ * 16-bit values, head_dim int8 codes or head_dim / 2 bytes; k_scale, v_scale [num_pages, num_kv_heads, page_size]
+ * (NULL for native pages); k_bounds [num_pages, num_kv_heads, 2, head_dim] 16-bit, the channel minima and maxima of every
+ * page's keys as they were given (NULL: not kept, sqattn_paged_select is refused).  page_size 16, 32, 64 or 128.
+ * Codes are symmetric: s = max(fl32(max|x| * fl32(1/Q)), 2^-100), Q = 127 or 7; code = nearest integer to x / s, ties to even;
+ * a row that holds an infinity or a NaN gets the scale NaN and reads back as NaN.
+ *
+ * A block table (device int32 [batch, max_pages], rows table_stride apart) names the page that holds tokens
+ * [i * page_size, (i + 1) * page_size) of a sequence.  Ids outside [0, num_pages) hold nothing: rows are not written
+ * there, read back as zeros and are left out of the attention; so are positions past max_pages * page_size. */
+typedef struct {
+  void *k_pages, *v_pages;
+  float *k_scale, *v_scale;
+  void* k_bounds;
+  int32_t num_pages, num_kv_heads, page_size, head_dim;
+  int32_t dtype;  /* of rows written and read, of queries, bounds and native pages */
+  int32_t format; /* SQATTN_KV_* */
+} sqattn_paged_pool;
+
+/* Write new rows: row i < counts[b] (counts NULL: i < num_rows) of k, v [B, Hkv, num_rows, D] becomes position
+ * positions[b] + i of sequence b (positions, counts: device int32 [B]; a negative position writes nothing for that
+ * sequence).  Position 0 of a page starts its bounds anew, later ones extend them.  Two sequences of one call must not
+ * write into the same page.  Rows 16-byte aligned. */
+int sqattn_paged_write(const sqattn_paged_pool* pool, const sqattn_tensor* k, const sqattn_tensor* v, int32_t batch,
+                       int32_t num_rows, const int32_t* block_table, int64_t table_stride, int32_t max_pages,
+                       const int32_t* positions, const int32_t* counts, sqattn_stream_t stream);
+/* Read rows back into k, v [B, Hkv, num_rows, D] 16-bit: row i of sequence b is position starts[b] + i, zeros where that is
+ * negative or at or past ends[b] (device int32 [B]; ends NULL: the table alone ends a sequence). */
+int sqattn_paged_read(const sqattn_paged_pool* pool, const sqattn_tensor_out* k, const sqattn_tensor_out* v, int32_t batch,
+                      int32_t num_rows, const int32_t* block_table, int64_t table_stride, int32_t max_pages,
+                      const int32_t* starts, const int32_t* ends, sqattn_stream_t stream);
+
+typedef struct {
+  const sqattn_paged_pool* pool;
+  sqattn_tensor q;            /* [B, Hq, 1, D] of the pool's dtype */
+  sqattn_tensor_out o;        /* [B, Hq, 1, D] */
+  float* lse;                 /* optional [B, Hq] fp32 base-2; -inf where a sequence has no keys (its output is 0) */
+  const int32_t* block_table; /* device [B, max_pages] */
+  int64_t table_stride;
+  const int32_t* kv_lens;     /* device [B]: read when the kernels run, so that a captured graph follows a growing cache */
+  const int32_t* pages;       /* device [B, Hkv, num_listed] pages of the sequence each KV head attends to (entries outside
+                                 [0, pages held) are skipped, one listed twice counts twice), or NULL: every page */
+  int32_t batch, num_q_heads, max_pages, num_listed, o_dtype;
+  int32_t max_kv_len;         /* 0, or a bound of kv_lens that the caller knows: longer sequences are cut there */
+  float sm_scale;             /* 0: 1/sqrt(head_dim) */
+  void* workspace;            /* sqattn_paged_decode_workspace_bytes() bytes, 256-byte aligned */
+  size_t workspace_bytes;
+} sqattn_paged_decode_args;
+
+/* o = softmax(sm_scale * q k^T) v over the first kv_lens[b] cached tokens (or those of them in the listed pages); at most
+ * 16 query heads per KV head.  Softmax statistics and sums in fp32, codes enter the products exactly. */
+size_t sqattn_paged_decode_workspace_bytes(const sqattn_paged_decode_args* args);
+int sqattn_paged_decode(const sqattn_paged_decode_args* args, sqattn_stream_t stream);
+
+/* Choose pages for sparse attention: per sequence and KV head the first sink_pages and last recent_pages pages it holds
+ * and, of the others, those with the highest sum_d max(u_d min_d, u_d max_d), u = the sum of the group's query heads, in
+ * fp64 (ties to the lowest page), budget in all.  out (device int32 [B, Hkv, budget]): ascending, -1 behind the last.
+ * budget >= sink_pages + recent_pages; max_pages <= 131072. */
+typedef struct {
+  const sqattn_paged_pool* pool;
+  sqattn_tensor q;            /* [B, Hq, 1, D] */
+  const int32_t* block_table;
+  int64_t table_stride;
+  const int32_t* kv_lens;     /* device [B] */
+  int32_t* out;
+  int32_t batch, num_q_heads, max_pages, budget, sink_pages, recent_pages;
+  void* workspace;            /* sqattn_paged_select_workspace_bytes() bytes, 256-byte aligned */
+  size_t workspace_bytes;
+} sqattn_paged_select_args;
+size_t sqattn_paged_select_workspace_bytes(const sqattn_paged_select_args* args);
+int sqattn_paged_select(const sqattn_paged_select_args* args, sqattn_stream_t stream);
+
 /* ---- diagnostics -------------------------------------------------------------------------- */
 
 /* Device-side waits (TMA / tensor-core completion barriers, the peer wait of the cross-GPU merge) are bounded; a

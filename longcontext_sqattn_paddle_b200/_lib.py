@@ -15,6 +15,7 @@ LIB_PATH = os.environ.get("SQATTN_B200_LIB") or os.path.join(_HERE, "libsqattn_b
 F16, BF16 = 0, 1
 MODE_DENSE_CAUSAL, MODE_RELATIVE_WINDOW, MODE_ABSOLUTE_WINDOW = 0, 1, 2
 P_FP8_OFF, P_FP8_ALL, P_FP8_STAGE2 = 0, 1, 2
+KV_FORMAT = {"native": 0, "int8": 1, "int4": 2}
 QTYPE = {"int": 0, "e4m3": 1, "e5m2": 2}
 
 OK, ERR_INVALID_ARG, ERR_UNSUPPORTED, ERR_CUDA, ERR_WORKSPACE, ERR_DEVICE_TIMEOUT = range(6)
@@ -95,6 +96,26 @@ class PeerMergeArgs(C.Structure):
                 ("lse", C.c_void_p)]
 
 
+class PagedPool(C.Structure):
+    _fields_ = [("k_pages", C.c_void_p), ("v_pages", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("k_bounds", C.c_void_p), ("num_pages", C.c_int32), ("num_kv_heads", C.c_int32), ("page_size", C.c_int32),
+                ("head_dim", C.c_int32), ("dtype", C.c_int32), ("format", C.c_int32)]
+
+
+class PagedDecodeArgs(C.Structure):
+    _fields_ = [("pool", C.c_void_p), ("q", Tensor), ("o", Tensor), ("lse", C.c_void_p), ("block_table", C.c_void_p),
+                ("table_stride", C.c_int64), ("kv_lens", C.c_void_p), ("pages", C.c_void_p), ("batch", C.c_int32),
+                ("num_q_heads", C.c_int32), ("max_pages", C.c_int32), ("num_listed", C.c_int32), ("o_dtype", C.c_int32),
+                ("max_kv_len", C.c_int32), ("sm_scale", C.c_float), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
+class PagedSelectArgs(C.Structure):
+    _fields_ = [("pool", C.c_void_p), ("q", Tensor), ("block_table", C.c_void_p), ("table_stride", C.c_int64),
+                ("kv_lens", C.c_void_p), ("out", C.c_void_p), ("batch", C.c_int32), ("num_q_heads", C.c_int32),
+                ("max_pages", C.c_int32), ("budget", C.c_int32), ("sink_pages", C.c_int32), ("recent_pages", C.c_int32),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
 SYMBOLS = [
     ("sqattn_prefill_workspace_bytes", C.c_size_t, [C.POINTER(PrefillArgs)]),
     ("sqattn_prefill", C.c_int, [C.POINTER(PrefillArgs), C.c_void_p]),
@@ -142,6 +163,14 @@ SYMBOLS = [
                                          C.c_void_p]),
     ("sqattn_cache_append", C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_int64,
                                       C.c_int64, C.c_int32, C.c_int32, C.c_int64, C.c_void_p]),
+    ("sqattn_paged_write", C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, C.c_void_p, C.c_int64, C.c_int32,
+                                     C.c_void_p, C.c_void_p, C.c_void_p]),
+    ("sqattn_paged_read", C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, C.c_void_p, C.c_int64, C.c_int32,
+                                    C.c_void_p, C.c_void_p, C.c_void_p]),
+    ("sqattn_paged_decode_workspace_bytes", C.c_size_t, [C.POINTER(PagedDecodeArgs)]),
+    ("sqattn_paged_decode", C.c_int, [C.POINTER(PagedDecodeArgs), C.c_void_p]),
+    ("sqattn_paged_select_workspace_bytes", C.c_size_t, [C.POINTER(PagedSelectArgs)]),
+    ("sqattn_paged_select", C.c_int, [C.POINTER(PagedSelectArgs), C.c_void_p]),
     ("sqattn_check_device_status", C.c_int, [C.c_void_p]),
     ("sqattn_set_status_mirror", C.c_int, [C.c_void_p]),
     ("sqattn_last_error_string", C.c_char_p, []),

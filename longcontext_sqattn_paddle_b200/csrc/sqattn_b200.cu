@@ -4,11 +4,16 @@
 #include <stdlib.h>
 #include <string.h>
 
+#include <algorithm>
+
 #include "common.cuh"
 #include "decode.cuh"
 #include "decoder_ops.cuh"
 #include "kmeans.cuh"
 #include "kmeans_tc.cuh"
+#include "paged_cache.cuh"
+#include "paged_decode.cuh"
+#include "paged_select.cuh"
 #include "peer_exchange.cuh"
 #include "prefill.cuh"
 #include "prep.cuh"
@@ -545,6 +550,89 @@ int launch_window_hist_tc(const WindowHistParams& p, int dtype, cudaStream_t str
   window_hist_tc_kernel<D><<<grid, kWtThreads, smem, stream>>>(tq, tk, p, dtype == SQATTN_BF16);
   SQ_CUDA(cudaGetLastError());
   return SQATTN_OK;
+}
+
+// ---- paged cache -------------------------------------------------------------------------------------------
+int paged_pool_check(const sqattn_paged_pool* p) {
+  if (!p) return fail(SQATTN_ERR_INVALID_ARG, "paged: pool is null");
+  if (p->head_dim != 64 && p->head_dim != 128) return fail(SQATTN_ERR_UNSUPPORTED, "paged: head_dim %d must be 64 or 128", p->head_dim);
+  if (p->page_size != 16 && p->page_size != 32 && p->page_size != 64 && p->page_size != 128)
+    return fail(SQATTN_ERR_UNSUPPORTED, "paged: page_size %d must be 16, 32, 64 or 128", p->page_size);
+  if (p->format < SQATTN_KV_NATIVE || p->format > SQATTN_KV_INT4) return fail(SQATTN_ERR_INVALID_ARG, "paged: unknown format %d", p->format);
+  if (p->dtype != SQATTN_F16 && p->dtype != SQATTN_BF16) return fail(SQATTN_ERR_INVALID_ARG, "paged: unknown dtype %d", p->dtype);
+  if (p->num_pages <= 0 || p->num_kv_heads <= 0 || p->num_kv_heads > 65535 ||
+      static_cast<int64_t>(p->num_pages) * p->num_kv_heads > 2147483647ll)
+    return fail(SQATTN_ERR_INVALID_ARG, "paged: %d pages of %d KV heads", p->num_pages, p->num_kv_heads);
+  if (!p->k_pages || !p->v_pages || (p->format != SQATTN_KV_NATIVE && (!p->k_scale || !p->v_scale)))
+    return fail(SQATTN_ERR_INVALID_ARG, "paged: null pool pointer");
+  if ((reinterpret_cast<uintptr_t>(p->k_pages) | reinterpret_cast<uintptr_t>(p->v_pages) | reinterpret_cast<uintptr_t>(p->k_scale) |
+       reinterpret_cast<uintptr_t>(p->v_scale) | reinterpret_cast<uintptr_t>(p->k_bounds)) & 15)
+    return fail(SQATTN_ERR_INVALID_ARG, "paged: pool tensors need 16-byte alignment");
+  return SQATTN_OK;
+}
+int paged_table_check(const int32_t* table, int64_t stride, int32_t max_pages, int32_t batch) {
+  if (batch <= 0 || batch > 65535) return fail(SQATTN_ERR_INVALID_ARG, "paged: batch %d must be 1..65535", batch);
+  if (!table || max_pages <= 0 || stride < 0) return fail(SQATTN_ERR_INVALID_ARG, "paged: block table of %d pages, row stride %lld", max_pages, static_cast<long long>(stride));
+  return SQATTN_OK;
+}
+PagedPool paged_pool(const sqattn_paged_pool* p) {
+  PagedPool r;
+  r.k_pages = static_cast<uint8_t*>(p->k_pages); r.v_pages = static_cast<uint8_t*>(p->v_pages);
+  r.k_scale = p->k_scale; r.v_scale = p->v_scale; r.k_bounds = static_cast<uint8_t*>(p->k_bounds);
+  r.num_pages = p->num_pages; r.hkv = p->num_kv_heads;
+  r.ps_shift = p->page_size == 16 ? 4 : p->page_size == 32 ? 5 : p->page_size == 64 ? 6 : 7;
+  return r;
+}
+bool rows16(const void* ptr, int64_t sb, int64_t sh, int64_t sn) {  // 16-byte pieces of every row can be moved whole
+  return reinterpret_cast<uintptr_t>(ptr) % 16 == 0 && sb % 8 == 0 && sh % 8 == 0 && sn % 8 == 0;
+}
+
+// KERNEL<format, head_dim, bf16> for a pool
+#define SQ_PAGED_DISPATCH(POOL, LAUNCH)                                                            \
+  do {                                                                                             \
+    const bool bf16_ = (POOL)->dtype == SQATTN_BF16;                                               \
+    if ((POOL)->head_dim == 128) {                                                                 \
+      if ((POOL)->format == SQATTN_KV_NATIVE) { if (bf16_) LAUNCH(kKvNative, 128, true); else LAUNCH(kKvNative, 128, false); } \
+      else if ((POOL)->format == SQATTN_KV_INT8) { if (bf16_) LAUNCH(kKvInt8, 128, true); else LAUNCH(kKvInt8, 128, false); } \
+      else { if (bf16_) LAUNCH(kKvInt4, 128, true); else LAUNCH(kKvInt4, 128, false); }            \
+    } else {                                                                                       \
+      if ((POOL)->format == SQATTN_KV_NATIVE) { if (bf16_) LAUNCH(kKvNative, 64, true); else LAUNCH(kKvNative, 64, false); } \
+      else if ((POOL)->format == SQATTN_KV_INT8) { if (bf16_) LAUNCH(kKvInt8, 64, true); else LAUNCH(kKvInt8, 64, false); } \
+      else { if (bf16_) LAUNCH(kKvInt4, 64, true); else LAUNCH(kKvInt4, 64, false); }              \
+    }                                                                                              \
+  } while (0)
+
+int paged_decode_check(const sqattn_paged_decode_args* a) {
+  if (!a) return fail(SQATTN_ERR_INVALID_ARG, "args is null");
+  int rc;
+  if ((rc = paged_pool_check(a->pool))) return rc;
+  if ((rc = paged_table_check(a->block_table, a->table_stride, a->max_pages, a->batch))) return rc;
+  if (a->num_q_heads <= 0 || a->num_q_heads % a->pool->num_kv_heads)
+    return fail(SQATTN_ERR_INVALID_ARG, "paged decode: %d query heads over %d KV heads", a->num_q_heads, a->pool->num_kv_heads);
+  if (a->num_q_heads / a->pool->num_kv_heads > 16)
+    return fail(SQATTN_ERR_UNSUPPORTED, "paged decode: at most 16 query heads per KV head, got %d", a->num_q_heads / a->pool->num_kv_heads);
+  if (!a->kv_lens) return fail(SQATTN_ERR_INVALID_ARG, "paged decode: kv_lens is null");
+  if (a->o_dtype != SQATTN_F16 && a->o_dtype != SQATTN_BF16) return fail(SQATTN_ERR_INVALID_ARG, "paged decode: unknown o_dtype %d", a->o_dtype);
+  if (a->max_kv_len < 0 || (a->pages && a->num_listed <= 0)) return fail(SQATTN_ERR_INVALID_ARG, "paged decode: max_kv_len %d, %d listed pages", a->max_kv_len, a->num_listed);
+  if (!(a->sm_scale >= 0.0f && a->sm_scale < 1e30f)) return fail(SQATTN_ERR_INVALID_ARG, "paged decode: sm_scale %g", a->sm_scale);
+  return SQATTN_OK;
+}
+
+int paged_select_check(const sqattn_paged_select_args* a) {
+  if (!a) return fail(SQATTN_ERR_INVALID_ARG, "args is null");
+  int rc;
+  if ((rc = paged_pool_check(a->pool))) return rc;
+  if ((rc = paged_table_check(a->block_table, a->table_stride, a->max_pages, a->batch))) return rc;
+  if (!a->pool->k_bounds) return fail(SQATTN_ERR_INVALID_ARG, "paged select: the pool keeps no key bounds");
+  if (a->max_pages > 131072) return fail(SQATTN_ERR_UNSUPPORTED, "paged select: %d pages a sequence, at most 131072", a->max_pages);
+  if (a->num_q_heads <= 0 || a->num_q_heads % a->pool->num_kv_heads)
+    return fail(SQATTN_ERR_INVALID_ARG, "paged select: %d query heads over %d KV heads", a->num_q_heads, a->pool->num_kv_heads);
+  if (a->sink_pages < 0 || a->recent_pages < 0 || a->budget <= 0 || a->budget - a->sink_pages < a->recent_pages)
+    return fail(SQATTN_ERR_INVALID_ARG, "paged select: %d pages in all, of which the first %d and the last %d", a->budget, a->sink_pages, a->recent_pages);
+  return SQATTN_OK;
+}
+size_t paged_select_ws(const sqattn_paged_select_args* a) {
+  return static_cast<size_t>(a->batch) * a->pool->num_kv_heads * a->max_pages * 8;
 }
 
 }  // namespace
@@ -1199,6 +1287,112 @@ int sqattn_cache_append(void* k_cache, void* v_cache, const void* k_new, const v
                                                 static_cast<const uint8_t*>(k_new), static_cast<const uint8_t*>(v_new),
                                                 reinterpret_cast<const long long*>(positions), cache_seq_stride,
                                                 cache_row_stride, new_seq_stride, batch, row_elems, capacity);
+  SQ_CUDA(cudaGetLastError());
+  return SQATTN_OK;
+}
+
+// ---- paged cache -------------------------------------------------------------------------------------------
+int sqattn_paged_write(const sqattn_paged_pool* pool, const sqattn_tensor* k, const sqattn_tensor* v, int32_t batch,
+                       int32_t num_rows, const int32_t* block_table, int64_t table_stride, int32_t max_pages,
+                       const int32_t* positions, const int32_t* counts, sqattn_stream_t stream_) {
+  cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
+  int rc;
+  if ((rc = paged_pool_check(pool)) || (rc = paged_table_check(block_table, table_stride, max_pages, batch))) return rc;
+  if (num_rows <= 0) return fail(SQATTN_ERR_INVALID_ARG, "paged write: %d rows", num_rows);
+  if (!k || !v || !k->ptr || !v->ptr || !positions) return fail(SQATTN_ERR_INVALID_ARG, "paged write: null pointer");
+  if (!rows16(k->ptr, k->stride_b, k->stride_h, k->stride_n) || !rows16(v->ptr, v->stride_b, v->stride_h, v->stride_n))
+    return fail(SQATTN_ERR_INVALID_ARG, "paged write: rows need 16-byte alignment");
+  PagedWriteParams p;
+  p.pool = paged_pool(pool);
+  p.table = {block_table, table_stride, max_pages};
+  p.k = static_cast<const uint8_t*>(k->ptr); p.v = static_cast<const uint8_t*>(v->ptr);
+  p.k_sb = k->stride_b; p.k_sh = k->stride_h; p.k_sn = k->stride_n;
+  p.v_sb = v->stride_b; p.v_sh = v->stride_h; p.v_sn = v->stride_n;
+  p.rows = num_rows; p.positions = positions; p.counts = counts;
+  const int64_t touched = (static_cast<int64_t>(num_rows) + pool->page_size - 2) / pool->page_size + 1;  // pages, wherever the rows start
+  const dim3 grid(static_cast<unsigned>(touched), pool->num_kv_heads, batch);
+#define SQ_LAUNCH(F, D, B) paged_write_kernel<F, D, B><<<grid, 128, 0, stream>>>(p)
+  SQ_PAGED_DISPATCH(pool, SQ_LAUNCH);
+#undef SQ_LAUNCH
+  SQ_CUDA(cudaGetLastError());
+  return SQATTN_OK;
+}
+
+int sqattn_paged_read(const sqattn_paged_pool* pool, const sqattn_tensor_out* k, const sqattn_tensor_out* v, int32_t batch,
+                      int32_t num_rows, const int32_t* block_table, int64_t table_stride, int32_t max_pages,
+                      const int32_t* starts, const int32_t* ends, sqattn_stream_t stream_) {
+  cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
+  int rc;
+  if ((rc = paged_pool_check(pool)) || (rc = paged_table_check(block_table, table_stride, max_pages, batch))) return rc;
+  if (num_rows <= 0) return fail(SQATTN_ERR_INVALID_ARG, "paged read: %d rows", num_rows);
+  if (!k || !v || !k->ptr || !v->ptr || !starts) return fail(SQATTN_ERR_INVALID_ARG, "paged read: null pointer");
+  if (!rows16(k->ptr, k->stride_b, k->stride_h, k->stride_n) || !rows16(v->ptr, v->stride_b, v->stride_h, v->stride_n))
+    return fail(SQATTN_ERR_INVALID_ARG, "paged read: rows need 16-byte alignment");
+  PagedReadParams p;
+  p.pool = paged_pool(pool);
+  p.table = {block_table, table_stride, max_pages};
+  p.k = static_cast<uint8_t*>(k->ptr); p.v = static_cast<uint8_t*>(v->ptr);
+  p.k_sb = k->stride_b; p.k_sh = k->stride_h; p.k_sn = k->stride_n;
+  p.v_sb = v->stride_b; p.v_sh = v->stride_h; p.v_sn = v->stride_n;
+  p.batch = batch; p.rows = num_rows; p.starts = starts; p.ends = ends;
+  const int grid = elementwise_grid(static_cast<long long>(batch) * num_rows * pool->num_kv_heads * (pool->head_dim / 8), 256);
+#define SQ_LAUNCH(F, D, B) paged_read_kernel<F, D, B><<<grid, 256, 0, stream>>>(p)
+  SQ_PAGED_DISPATCH(pool, SQ_LAUNCH);
+#undef SQ_LAUNCH
+  SQ_CUDA(cudaGetLastError());
+  return SQATTN_OK;
+}
+
+size_t sqattn_paged_decode_workspace_bytes(const sqattn_paged_decode_args* a) {
+  if (paged_decode_check(a)) return 0;
+  return 256;
+}
+
+int sqattn_paged_decode(const sqattn_paged_decode_args* a, sqattn_stream_t stream_) {
+  cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
+  int rc;
+  if ((rc = paged_decode_check(a))) return rc;
+  if (!a->q.ptr || !a->o.ptr) return fail(SQATTN_ERR_INVALID_ARG, "paged decode: null tensor pointer");
+  if ((reinterpret_cast<uintptr_t>(a->q.ptr) | reinterpret_cast<uintptr_t>(a->o.ptr)) & 1) return fail(SQATTN_ERR_INVALID_ARG, "paged decode: q and o need 2-byte alignment");
+  PagedDecodeParams p;
+  memset(&p, 0, sizeof(p));
+  p.pool = paged_pool(a->pool);
+  p.table = {a->block_table, a->table_stride, a->max_pages};
+  p.q = static_cast<const uint8_t*>(a->q.ptr); p.q_sb = a->q.stride_b; p.q_sh = a->q.stride_h;
+  p.o = static_cast<uint8_t*>(a->o.ptr); p.o_sb = a->o.stride_b; p.o_sh = a->o.stride_h;
+  p.lse = a->lse; p.kv_lens = a->kv_lens; p.list = a->pages; p.list_len = a->num_listed;
+  p.max_len = static_cast<int>(std::min<int64_t>(static_cast<int64_t>(a->max_pages) * a->pool->page_size, a->max_kv_len ? a->max_kv_len : 2147483647));
+  p.batch = a->batch; p.hq = a->num_q_heads; p.groups = a->num_q_heads / a->pool->num_kv_heads; p.o_bf16 = a->o_dtype == SQATTN_BF16;
+  p.scale_log2 = static_cast<float>((a->sm_scale > 0.0f ? static_cast<double>(a->sm_scale) : 1.0 / sqrt(static_cast<double>(a->pool->head_dim))) * 1.4426950408889634);
+#define SQ_LAUNCH(F, D, B) paged_decode_kernel<F, D, B><<<dim3(a->num_q_heads, a->batch), 256, 0, stream>>>(p)
+  SQ_PAGED_DISPATCH(a->pool, SQ_LAUNCH);
+#undef SQ_LAUNCH
+  SQ_CUDA(cudaGetLastError());
+  return SQATTN_OK;
+}
+
+size_t sqattn_paged_select_workspace_bytes(const sqattn_paged_select_args* a) { return paged_select_check(a) ? 0 : paged_select_ws(a); }
+
+int sqattn_paged_select(const sqattn_paged_select_args* a, sqattn_stream_t stream_) {
+  cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
+  int rc;
+  if ((rc = paged_select_check(a))) return rc;
+  if (!a->q.ptr || !a->kv_lens || !a->out) return fail(SQATTN_ERR_INVALID_ARG, "paged select: null pointer");
+  if (reinterpret_cast<uintptr_t>(a->q.ptr) & 1) return fail(SQATTN_ERR_INVALID_ARG, "paged select: q needs 2-byte alignment");
+  if (!a->workspace || a->workspace_bytes < paged_select_ws(a) || (reinterpret_cast<uintptr_t>(a->workspace) % 256))
+    return fail(SQATTN_ERR_WORKSPACE, "workspace of %zu bytes (256-byte aligned) required", paged_select_ws(a));
+  PagedSelectParams p;
+  p.pool = paged_pool(a->pool);
+  p.table = {a->block_table, a->table_stride, a->max_pages};
+  p.q = static_cast<const uint8_t*>(a->q.ptr); p.q_sb = a->q.stride_b; p.q_sh = a->q.stride_h;
+  p.kv_lens = a->kv_lens; p.batch = a->batch; p.groups = a->num_q_heads / a->pool->num_kv_heads;
+  p.budget = a->budget; p.sink_pages = a->sink_pages; p.recent_pages = a->recent_pages;
+  p.keys = static_cast<unsigned long long*>(a->workspace); p.out = a->out;
+  const dim3 grid((a->max_pages + 255) / 256, a->pool->num_kv_heads, a->batch);
+  const bool bf16 = a->pool->dtype == SQATTN_BF16;
+  if (a->pool->head_dim == 128) { if (bf16) paged_score_kernel<128, true><<<grid, 256, 0, stream>>>(p); else paged_score_kernel<128, false><<<grid, 256, 0, stream>>>(p); }
+  else { if (bf16) paged_score_kernel<64, true><<<grid, 256, 0, stream>>>(p); else paged_score_kernel<64, false><<<grid, 256, 0, stream>>>(p); }
+  paged_pick_kernel<<<dim3(a->pool->num_kv_heads, a->batch), 1024, 0, stream>>>(p);
   SQ_CUDA(cudaGetLastError());
   return SQATTN_OK;
 }

@@ -55,6 +55,9 @@ _PREP_ARGS = struct.Struct("4q4q4q5q10iqQqii")
 assert _PREFILL_ARGS.size == C.sizeof(L.PrefillArgs) and _PREP_ARGS.size == C.sizeof(L.PrepArgs)
 _DECODE_ARGS = struct.Struct("4q4q4q4qq5i4xq6iqQqqqqi4xq")
 assert _DECODE_ARGS.size == C.sizeof(L.DecodeArgs)
+_PAGED_DECODE_ARGS = struct.Struct("q4q4qqqqqq6if4xqQ")
+_PAGED_SELECT_ARGS = struct.Struct("q4qqqqq6iqQ")
+assert _PAGED_DECODE_ARGS.size == C.sizeof(L.PagedDecodeArgs) and _PAGED_SELECT_ARGS.size == C.sizeof(L.PagedSelectArgs)
 
 
 def _decode_args(q, k, v, o, lse, batch, hq, hkv, d, kv_len, dtype, o_dtype, *, kv_lens=0, p_fp8=False, q_is_scaled=False, num_splits=0,
@@ -426,4 +429,182 @@ def silu_mul(x: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tenso
     out = torch.empty(*x.shape[:-1], inter, dtype=x.dtype, device=x.device) if out is None else out
     assert out.is_contiguous()
     L.check(L.lib.sqattn_silu_mul(x.data_ptr(), out.data_ptr(), x.numel() // (2 * inter), inter, _dt(x.dtype), _stream()))
+    return out
+
+
+# ---- paged key/value cache -------------------------------------------------------------------------------------------
+PAGE_SIZES = (16, 32, 64, 128)
+
+
+class PagedPool:
+    """One layer's pages of a key/value cache (sqattn_paged_pool): ``k_pages`` / ``v_pages`` [pages, Hkv, page_size, row] with
+    a row of D values of ``dtype`` ("native"), D int8 codes ("int8") or D / 2 bytes of two 4-bit codes ("int4"); ``k_scale`` /
+    ``v_scale`` [pages, Hkv, page_size] fp32 for codes; ``k_bounds`` [pages, Hkv, 2, D] of ``dtype`` (channel minima and maxima
+    of every page's keys, None: not kept).  The format follows from the pages' type.  All tensors contiguous on one GPU."""
+
+    __slots__ = ("k_pages", "v_pages", "k_scale", "v_scale", "k_bounds", "dtype", "kv_format", "num_pages", "num_kv_heads",
+                 "page_size", "head_dim", "device", "_struct", "_address")
+
+    def __init__(self, k_pages, v_pages, k_scale=None, v_scale=None, k_bounds=None, dtype=None):
+        kinds = {torch.int8: "int8", torch.uint8: "int4"}
+        self.kv_format = kinds.get(k_pages.dtype, "native")
+        self.dtype = k_pages.dtype if dtype is None else dtype
+        code = _dt(self.dtype)
+        if k_pages.dim() != 4 or v_pages.shape != k_pages.shape or v_pages.dtype != k_pages.dtype:
+            raise ValueError(f"k_pages and v_pages must both be [pages, Hkv, page_size, row] of one type, got {tuple(k_pages.shape)} "
+                             f"{k_pages.dtype} and {tuple(v_pages.shape)} {v_pages.dtype}")
+        if self.kv_format == "native" and k_pages.dtype != self.dtype:
+            raise ValueError(f"native pages hold {self.dtype}, got {k_pages.dtype}")
+        self.num_pages, self.num_kv_heads, self.page_size, row = k_pages.shape
+        self.head_dim = 2 * row if self.kv_format == "int4" else row
+        if self.page_size not in PAGE_SIZES:
+            raise ValueError(f"page_size {self.page_size} must be one of {PAGE_SIZES}")
+        if self.head_dim not in (64, 128):
+            raise ValueError(f"head_dim {self.head_dim} must be 64 or 128")
+        if (k_scale is None) != (self.kv_format == "native") or (v_scale is None) != (k_scale is None):
+            raise ValueError(f"{self.kv_format} pages {'take no' if self.kv_format == 'native' else 'need k_scale and v_scale'} scales")
+        self.k_pages, self.v_pages, self.k_scale, self.v_scale, self.k_bounds = k_pages, v_pages, k_scale, v_scale, k_bounds
+        self.device = k_pages.device
+        for t, shape, kind, name in ((k_scale, k_pages.shape[:3], torch.float32, "k_scale"),
+                                     (v_scale, k_pages.shape[:3], torch.float32, "v_scale"),
+                                     (k_bounds, (self.num_pages, self.num_kv_heads, 2, self.head_dim), self.dtype, "k_bounds")):
+            if t is not None and (t.shape != shape or t.dtype != kind):
+                raise ValueError(f"{name} must be {tuple(shape)} {kind}, got {tuple(t.shape)} {t.dtype}")
+        given = [t for t in (k_pages, v_pages, k_scale, v_scale, k_bounds) if t is not None]
+        _require_cuda(*given)
+        if any(not t.is_contiguous() or t.device != self.device or t.data_ptr() % 16 for t in given):
+            raise ValueError("a pool's tensors must be contiguous, 16-byte aligned and on one device")
+        self._struct = L.PagedPool(*(0 if t is None else t.data_ptr() for t in (k_pages, v_pages, k_scale, v_scale, k_bounds)),
+                                   self.num_pages, self.num_kv_heads, self.page_size, self.head_dim, code, L.KV_FORMAT[self.kv_format])
+        self._address = C.addressof(self._struct)
+
+    @classmethod
+    def allocate(cls, num_pages: int, page_size: int, num_kv_heads: int, head_dim: int, dtype=torch.bfloat16,
+                 kv_format: str = "int8", bounds: bool = True, device="cuda") -> "PagedPool":
+        """A pool of empty pages."""
+        if kv_format not in L.KV_FORMAT:
+            raise ValueError(f"kv_format {kv_format} must be one of {tuple(L.KV_FORMAT)}")
+        kind = {"native": dtype, "int8": torch.int8, "int4": torch.uint8}[kv_format]
+        shape = (num_pages, num_kv_heads, page_size)
+        row = head_dim // 2 if kv_format == "int4" else head_dim
+        pages = [torch.empty(*shape, row, dtype=kind, device=device) for _ in range(2)]
+        scales = [None if kv_format == "native" else torch.empty(shape, dtype=torch.float32, device=device) for _ in range(2)]
+        k_bounds = torch.zeros(num_pages, num_kv_heads, 2, head_dim, dtype=dtype, device=device) if bounds else None
+        return cls(*pages, *scales, k_bounds, dtype=dtype)
+
+
+def _paged_index(pool: PagedPool, block_table, batch: int, **ints):
+    """Check the index tensors of a paged call: int32, on the pool's device, one entry a sequence."""
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != batch or block_table.device != pool.device or \
+            (block_table.shape[1] > 1 and block_table.stride(1) != 1):
+        raise ValueError(f"block_table must be int32 [{batch}, max_pages] with contiguous rows on {pool.device}, got "
+                         f"{tuple(block_table.shape)} {block_table.dtype} on {block_table.device}")
+    for name, t in ints.items():
+        if t is not None and (t.dtype != torch.int32 or t.shape != (batch,) or t.device != pool.device or not t.is_contiguous()):
+            raise ValueError(f"{name} must be a contiguous int32 [{batch}] on {pool.device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
+
+
+def _paged_rows(pool: PagedPool, t, name: str):
+    """New rows [B, N, Hkv, D] as the kernels read them: 16-byte pieces, copied only where the strides do not allow that."""
+    if t.dim() != 4 or t.shape[2] != pool.num_kv_heads or t.shape[3] != pool.head_dim or t.dtype != pool.dtype or t.device != pool.device:
+        raise ValueError(f"{name} must be [B, N, {pool.num_kv_heads}, {pool.head_dim}] {pool.dtype} on {pool.device}, got "
+                         f"{tuple(t.shape)} {t.dtype} on {t.device}")
+    st = t.stride()
+    if st[3] != 1 or t.data_ptr() % 16 or (st[0] | st[1] | st[2]) % 8:
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def _paged_query(pool: PagedPool, q, layout: str):
+    """Descriptor and head count of a query [B, 1, Hq, D] (NHD) or [B, Hq, 1, D] (HND)."""
+    if q.dim() != 4 or q.dtype != pool.dtype or q.device != pool.device or q.shape[3] != pool.head_dim or q.stride(3) != 1:
+        raise ValueError(f"the query must have 4 dimensions, a contiguous last one of {pool.head_dim}, be {pool.dtype} and on {pool.device}, got "
+                         f"{tuple(q.shape)} {q.dtype} on {q.device}")
+    desc = _desc(q, layout)
+    b, hq, one, _ = _shape(q, layout)
+    if one != 1:
+        raise ValueError(f"one query token a sequence, got {one}")
+    return desc, b, hq
+
+
+def paged_write(pool: PagedPool, key, value, block_table, positions, counts=None) -> None:
+    """sqattn_paged_write: quantise new rows into pages.  key / value [B, N, Hkv, D] (any strides) become positions
+    ``positions[b] ...`` of the sequences whose pages ``block_table`` [B, max_pages] names; of each only the first
+    ``counts[b]`` rows (int32 [B], None: all N).  Two sequences of one call must not write into the same page."""
+    if key.shape != value.shape:
+        raise ValueError(f"key and value must have one shape, got {tuple(key.shape)} and {tuple(value.shape)}")
+    key, value = _paged_rows(pool, key, "key"), _paged_rows(pool, value, "value")
+    b, n = key.shape[:2]
+    _paged_index(pool, block_table, b, positions=positions, counts=counts)
+    if b == 0 or n == 0:
+        return
+    kd, vd = L.Tensor(*_desc(key, "NHD")), L.Tensor(*_desc(value, "NHD"))
+    with torch.cuda.device(pool.device):
+        L.check(L.lib.sqattn_paged_write(pool._address, C.addressof(kd), C.addressof(vd), b, n, block_table.data_ptr(), block_table.stride(0),
+                                         block_table.shape[1], positions.data_ptr(), None if counts is None else counts.data_ptr(), _stream()))
+
+
+def paged_read(pool: PagedPool, block_table, starts, num_rows: int, ends=None, out=None):
+    """sqattn_paged_read: (key, value) [B, num_rows, Hkv, D] of positions ``starts[b] + i``, zeros at or past ``ends[b]``
+    (int32 [B]; None: where the block table ends).  ``out``: a pair of tensors to write into (16-byte aligned rows)."""
+    b = block_table.shape[0]
+    _paged_index(pool, block_table, b, starts=starts, ends=ends)
+    shape = (b, int(num_rows), pool.num_kv_heads, pool.head_dim)
+    if out is None:
+        out = tuple(torch.empty(shape, dtype=pool.dtype, device=pool.device) for _ in range(2))
+    else:
+        for t in out:
+            st = t.stride()
+            if t.shape != shape or t.dtype != pool.dtype or t.device != pool.device or st[3] != 1 or t.data_ptr() % 16 or (st[0] | st[1] | st[2]) % 8:
+                raise ValueError(f"out must be two {shape} {pool.dtype} tensors on {pool.device} with 16-byte aligned rows")
+            if any(ext > 1 and s == 0 for s, ext in zip(st, t.shape)):
+                raise ValueError("out must not be a broadcast view")
+    if b == 0 or num_rows == 0:
+        return out
+    kd, vd = (L.Tensor(*_desc(t, "NHD")) for t in out)
+    with torch.cuda.device(pool.device):
+        L.check(L.lib.sqattn_paged_read(pool._address, C.addressof(kd), C.addressof(vd), b, int(num_rows), block_table.data_ptr(),
+                                        block_table.stride(0), block_table.shape[1], starts.data_ptr(),
+                                        None if ends is None else ends.data_ptr(), _stream()))
+    return out
+
+
+def paged_decode(q, pool: PagedPool, block_table, kv_lens, *, pages=None, max_kv_len: int = 0, sm_scale: float = 0.0,
+                 layout: str = "NHD", out_dtype=None, return_lse: bool = False):
+    """sqattn_paged_decode: one query token per sequence, q [B, 1, Hq, D] (NHD) or [B, Hq, 1, D] (HND), against its first
+    ``kv_lens[b]`` cached tokens (int32 [B] on the device, read when the kernels run).  ``pages`` int32 [B, Hkv, n]: only the
+    listed pages of the sequence (``paged_select`` makes such a list).  ``max_kv_len``: a bound of the lengths, if the caller
+    knows one below the block table's (0: none).  A sequence without keys gets zeros and an LSE of -inf."""
+    poll_device_status(pool.device)
+    qd, b, hq = _paged_query(pool, q, layout)
+    _paged_index(pool, block_table, b, kv_lens=kv_lens)
+    if pages is not None and (pages.dtype != torch.int32 or pages.dim() != 3 or pages.shape[:2] != (b, pool.num_kv_heads) or
+                              not pages.is_contiguous() or pages.device != pool.device):
+        raise ValueError(f"pages must be a contiguous int32 [{b}, {pool.num_kv_heads}, n] on {pool.device}, got {tuple(pages.shape)} {pages.dtype}")
+    out = torch.empty(q.shape, dtype=out_dtype or pool.dtype, device=q.device)
+    lse = torch.empty(b, hq, 1, dtype=torch.float32, device=q.device) if return_lse else None
+    if b:
+        a = L.PagedDecodeArgs.from_buffer(bytearray(_PAGED_DECODE_ARGS.pack(
+            pool._address, *qd, *_desc(out, layout), 0 if lse is None else lse.data_ptr(), block_table.data_ptr(), block_table.stride(0),
+            kv_lens.data_ptr(), 0 if pages is None else pages.data_ptr(), b, hq, block_table.shape[1],
+            0 if pages is None else pages.shape[2], _dt(out.dtype), int(max_kv_len), float(sm_scale), 0, 0)))
+        with torch.cuda.device(pool.device):
+            _run_decode(a, q.device, L.lib.sqattn_paged_decode_workspace_bytes, L.lib.sqattn_paged_decode)
+    return (out, lse) if return_lse else out
+
+
+def paged_select(q, pool: PagedPool, block_table, kv_lens, num_pages: int, *, sink_pages: int = 1, recent_pages: int = 1,
+                 layout: str = "NHD"):
+    """sqattn_paged_select: int32 [B, Hkv, num_pages], the pages of each sequence that a KV head's query group should attend
+    to, ascending, -1 behind the last: the first ``sink_pages``, the last ``recent_pages`` and those whose key bounds allow the
+    highest scores."""
+    qd, b, hq = _paged_query(pool, q, layout)
+    _paged_index(pool, block_table, b, kv_lens=kv_lens)
+    out = torch.empty(b, pool.num_kv_heads, int(num_pages), dtype=torch.int32, device=q.device)
+    if b:
+        a = L.PagedSelectArgs.from_buffer(bytearray(_PAGED_SELECT_ARGS.pack(
+            pool._address, *qd, block_table.data_ptr(), block_table.stride(0), kv_lens.data_ptr(), out.data_ptr(), b, hq,
+            block_table.shape[1], int(num_pages), int(sink_pages), int(recent_pages), 0, 0)))
+        with torch.cuda.device(pool.device):
+            _run_decode(a, q.device, L.lib.sqattn_paged_select_workspace_bytes, L.lib.sqattn_paged_select)
     return out

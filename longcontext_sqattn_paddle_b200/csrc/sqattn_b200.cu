@@ -618,6 +618,67 @@ int paged_decode_check(const sqattn_paged_decode_args* a) {
   return SQATTN_OK;
 }
 
+// scratch of a paged decode: [part_o | part_lse | plan]
+struct PagedDecodePlan {
+  int grid, min_tiles, max_len;
+  size_t parts, lse_off, plan_off, total;
+};
+int plan_paged_decode(const sqattn_paged_decode_args* a, PagedDecodePlan* pl) {
+  int rc;
+  if ((rc = paged_decode_check(a))) return rc;
+  const sqattn_paged_pool* pool = a->pool;
+  if (a->batch > kPagedMaxBatch) return fail(SQATTN_ERR_UNSUPPORTED, "paged decode: at most %d sequences a call, got %d", kPagedMaxBatch, a->batch);
+  const int64_t cap = std::min<int64_t>(static_cast<int64_t>(a->max_pages) * pool->page_size, 0x7fffff00ll);
+  pl->max_len = static_cast<int>(a->max_kv_len ? std::min<int64_t>(cap, a->max_kv_len) : cap);
+  const int64_t keys = a->pages ? static_cast<int64_t>(a->num_listed) * pool->page_size : pl->max_len;
+  const int64_t tiles = (keys + kPagedTile - 1) / kPagedTile * pool->num_kv_heads;
+  if (keys > 0x7fffff00ll || tiles > 2147483647ll / a->batch)
+    return fail(SQATTN_ERR_UNSUPPORTED, "paged decode: %d sequences of up to %lld keys and %d KV heads are more than a call takes (max_kv_len bounds the keys)",
+                a->batch, static_cast<long long>(keys), pool->num_kv_heads);
+  pl->min_tiles = (pool->format == SQATTN_KV_NATIVE && pool->head_dim == 128) ? 4 : 8;   // one for each warp
+  pl->grid = static_cast<int>(std::min<int64_t>(148, (tiles * a->batch + pl->min_tiles - 1) / pl->min_tiles));   // one CTA per SM
+  const int groups = a->num_q_heads / pool->num_kv_heads;
+  pl->parts = static_cast<size_t>(pl->grid) + static_cast<size_t>(a->batch) * pool->num_kv_heads;
+  pl->lse_off = align_up(pl->parts * groups * pool->head_dim * 4, 256);
+  pl->plan_off = pl->lse_off + align_up(pl->parts * groups * 4, 256);
+  pl->total = pl->plan_off + align_up((static_cast<size_t>(a->batch) + 2) * 4, 256);
+  return SQATTN_OK;
+}
+
+// Pages of a pool as 128-byte lines: dimensions (128 bytes, lines of a page and head, halves of a row, page * Hkv + head).  Rows of
+// 256 bytes are two halves, so that the 128-byte swizzle spreads the rows of a half over the banks; shorter rows lie behind
+// one another.
+int make_tmap_pages(CUtensorMap* out, const void* ptr, const sqattn_paged_pool* pool, int row_bytes, int box_rows, const char* name) {
+  EncodeTiledFn fn = encode_tiled_fn();
+  if (!fn) return fail(SQATTN_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
+  const int halves = row_bytes == 256 ? 2 : 1;
+  const cuuint64_t block = static_cast<cuuint64_t>(pool->page_size) * row_bytes;
+  cuuint64_t dims[4] = {128, block / 128 / halves, static_cast<cuuint64_t>(halves), static_cast<cuuint64_t>(pool->num_pages) * pool->num_kv_heads};
+  cuuint64_t strides[3] = {static_cast<cuuint64_t>(128 * halves), 128, block};
+  cuuint32_t box[4] = {128, static_cast<cuuint32_t>(box_rows * row_bytes / 128 / halves), static_cast<cuuint32_t>(halves), 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(SQATTN_ERR_CUDA, "%s: cuTensorMapEncodeTiled failed (%d)", name, static_cast<int>(r));
+  return SQATTN_OK;
+}
+
+template <int FMT, int D, bool BF16, int NT>
+int launch_paged_decode(const sqattn_paged_decode_args* a, const PagedDecodePlan& pl, const PagedDecodeParams& p, cudaStream_t stream) {
+  using Cfg = PagedDecodeCfg<FMT, D, NT>;
+  const int box_rows = (FMT == kKvNative || a->pool->page_size == 16) ? 16 : 32;
+  CUtensorMap tk, tv;
+  int rc;
+  if ((rc = make_tmap_pages(&tk, a->pool->k_pages, a->pool, Cfg::kRow, box_rows, "k_pages"))) return rc;
+  if ((rc = make_tmap_pages(&tv, a->pool->v_pages, a->pool, Cfg::kRow, box_rows, "v_pages"))) return rc;
+  SQ_CUDA(cudaFuncSetAttribute(paged_decode_kernel<FMT, D, BF16, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::total(a->batch)));
+  paged_decode_kernel<FMT, D, BF16, NT><<<pl.grid, Cfg::kWarps * 32, Cfg::total(a->batch), stream>>>(tk, tv, p);
+  SQ_CUDA(cudaGetLastError());
+  if (pl.grid > 1)
+    SQ_CUDA(launch_overlapped(1, paged_merge_kernel<D>, dim3(a->num_q_heads, a->batch), dim3(128 * kMergeGroups), 0, stream, p));
+  return SQATTN_OK;
+}
+
 int paged_select_check(const sqattn_paged_select_args* a) {
   if (!a) return fail(SQATTN_ERR_INVALID_ARG, "args is null");
   int rc;
@@ -1344,30 +1405,41 @@ int sqattn_paged_read(const sqattn_paged_pool* pool, const sqattn_tensor_out* k,
 }
 
 size_t sqattn_paged_decode_workspace_bytes(const sqattn_paged_decode_args* a) {
-  if (paged_decode_check(a)) return 0;
-  return 256;
+  PagedDecodePlan pl;
+  return plan_paged_decode(a, &pl) ? 0 : pl.total;
 }
 
 int sqattn_paged_decode(const sqattn_paged_decode_args* a, sqattn_stream_t stream_) {
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
+  PagedDecodePlan pl;
   int rc;
-  if ((rc = paged_decode_check(a))) return rc;
+  if ((rc = plan_paged_decode(a, &pl))) return rc;
+  const sqattn_paged_pool* pool = a->pool;
   if (!a->q.ptr || !a->o.ptr) return fail(SQATTN_ERR_INVALID_ARG, "paged decode: null tensor pointer");
   if ((reinterpret_cast<uintptr_t>(a->q.ptr) | reinterpret_cast<uintptr_t>(a->o.ptr)) & 1) return fail(SQATTN_ERR_INVALID_ARG, "paged decode: q and o need 2-byte alignment");
+  if (!a->workspace || a->workspace_bytes < pl.total || (reinterpret_cast<uintptr_t>(a->workspace) % 256))
+    return fail(SQATTN_ERR_WORKSPACE, "workspace of %zu bytes (256-byte aligned) required", pl.total);
   PagedDecodeParams p;
   memset(&p, 0, sizeof(p));
-  p.pool = paged_pool(a->pool);
+  p.pool = paged_pool(pool);
   p.table = {a->block_table, a->table_stride, a->max_pages};
   p.q = static_cast<const uint8_t*>(a->q.ptr); p.q_sb = a->q.stride_b; p.q_sh = a->q.stride_h;
   p.o = static_cast<uint8_t*>(a->o.ptr); p.o_sb = a->o.stride_b; p.o_sh = a->o.stride_h;
   p.lse = a->lse; p.kv_lens = a->kv_lens; p.list = a->pages; p.list_len = a->num_listed;
-  p.max_len = static_cast<int>(std::min<int64_t>(static_cast<int64_t>(a->max_pages) * a->pool->page_size, a->max_kv_len ? a->max_kv_len : 2147483647));
-  p.batch = a->batch; p.hq = a->num_q_heads; p.groups = a->num_q_heads / a->pool->num_kv_heads; p.o_bf16 = a->o_dtype == SQATTN_BF16;
-  p.scale_log2 = static_cast<float>((a->sm_scale > 0.0f ? static_cast<double>(a->sm_scale) : 1.0 / sqrt(static_cast<double>(a->pool->head_dim))) * 1.4426950408889634);
-#define SQ_LAUNCH(F, D, B) paged_decode_kernel<F, D, B><<<dim3(a->num_q_heads, a->batch), 256, 0, stream>>>(p)
-  SQ_PAGED_DISPATCH(a->pool, SQ_LAUNCH);
+  p.max_len = pl.max_len; p.min_tiles = pl.min_tiles;
+  p.batch = a->batch; p.hq = a->num_q_heads; p.groups = a->num_q_heads / pool->num_kv_heads;
+  p.q_bf16 = pool->dtype == SQATTN_BF16; p.o_bf16 = a->o_dtype == SQATTN_BF16;
+  const double scale = a->sm_scale > 0.0f ? static_cast<double>(a->sm_scale) : 1.0 / sqrt(static_cast<double>(pool->head_dim));
+  p.scale_log2 = std::max(static_cast<float>(scale * 1.4426950408889634), 1e-30f);   // a factor of 0 would turn masked scores into NaN
+  uint8_t* ws = static_cast<uint8_t*>(a->workspace);
+  p.part_o = reinterpret_cast<float*>(ws);
+  p.part_lse = reinterpret_cast<float*>(ws + pl.lse_off);
+  p.plan = reinterpret_cast<int*>(ws + pl.plan_off);
+  // codes become f16 whatever the queries' type
+#define SQ_LAUNCH(F, D, B) \
+  return p.groups > 8 ? launch_paged_decode<F, D, (F) == kKvNative && B, 2>(a, pl, p, stream) : launch_paged_decode<F, D, (F) == kKvNative && B, 1>(a, pl, p, stream)
+  SQ_PAGED_DISPATCH(pool, SQ_LAUNCH);
 #undef SQ_LAUNCH
-  SQ_CUDA(cudaGetLastError());
   return SQATTN_OK;
 }
 
@@ -1406,7 +1478,7 @@ int sqattn_check_device_status(sqattn_stream_t stream_) {
   if (code != 0) {
     const int zero = 0;
     cudaMemcpyToSymbolAsync(g_device_status, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, stream);
-    return fail(SQATTN_ERR_DEVICE_TIMEOUT, "a device-side wait gave up (code %d: 1xx prefill, 2xx decode)", code);
+    return fail(SQATTN_ERR_DEVICE_TIMEOUT, "a device-side wait gave up (code %d: 1xx prefill, 2xx decode, 4xx paged decode)", code);
   }
   return SQATTN_OK;
 }

@@ -105,7 +105,7 @@ def poll_device_status(device=None):
     code = ent[1].value
     if code:
         raise L.SqattnError(L.ERR_DEVICE_TIMEOUT, f"a device-side wait gave up on cuda:{idx} (code {code}: 1xx prefill, "
-                            "2xx decode, 3xx peer exchange); outputs since then are NaN; call check_device_status() to clear")
+                            "2xx decode, 3xx peer exchange, 4xx paged decode); outputs since then are NaN; call check_device_status() to clear")
 
 
 def _workspace(nbytes: int, device) -> Optional[torch.Tensor]:

@@ -89,14 +89,14 @@ def read(pool, fmt, dtype, table, starts, n, ends):
 
 def attention(q, pool, fmt, table, lens, pages=None, sm_scale=None):
     """q [B, Hq, D] -> (o [B, Hq, D] fp64, lse [B, Hq] fp64 base 2, spread [B, Hq, D] = sum_j p_j |v_j|, size [B, Hq] =
-    max_j sm_scale sum_d |q_d k_jd|): the last two are what error bounds are made of."""
+    max_j sm_scale sum_d |q_d k_jd|, vmax [B, Hq] = max |v|): the last three are what error bounds are made of."""
     b, hq, d = q.shape
     num_pages, hkv, ps = pool["k_pages"].shape[:3]
     g = hq // hkv
     sm_scale = 1.0 / math.sqrt(d) if sm_scale is None else sm_scale
     o = torch.zeros(b, hq, d, dtype=torch.float64, device=q.device)
     lse = torch.full((b, hq), -float("inf"), dtype=torch.float64, device=q.device)
-    spread, size = torch.zeros_like(o), torch.zeros_like(lse)
+    spread, size, vmax = torch.zeros_like(o), torch.zeros_like(lse), torch.zeros_like(lse)
     for i in range(b):
         n = max(0, min(lens[i], table.shape[1] * ps))
         held = (n + ps - 1) // ps
@@ -117,8 +117,9 @@ def attention(q, pool, fmt, table, lens, pages=None, sm_scale=None):
             o[i, h * g:(h + 1) * g] = w @ v
             spread[i, h * g:(h + 1) * g] = w @ v.abs()
             size[i, h * g:(h + 1) * g] = (x.abs() @ k.abs().T * sm_scale).amax(-1)
+            vmax[i, h * g:(h + 1) * g] = v.abs().amax()
             lse[i, h * g:(h + 1) * g] = torch.logsumexp(s, -1) / math.log(2.0)
-    return o, lse, spread, size
+    return o, lse, spread, size, vmax
 
 
 def select(q, pool, table, lens, budget, sink, recent):

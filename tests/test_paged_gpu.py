@@ -206,13 +206,18 @@ def test_write_and_read_take_strided_and_unaligned_tensors():
 def _check_attention(q, pool, fmt, table, lens, out, lse, pages=None, sm_scale=None):
     """|o - ref| <= half a step of the output's type + errors of the weights: their rounding to 11 bits, of the scores
     (sums of D products in fp32, so D steps of 2^-23 of sum |q k|; both numerator and denominator have it) and of sums of n
-    terms in fp32.  The LSE has the scores' and the sum's."""
+    terms in fp32.  The LSE has the scores' and the sum's.
+
+    A weight p s_j (s_j the value's scale, p <= 1) is rounded to f16 as p s_j 2^14 / 2^e with 2^e <= max s, so below f16's
+    normal numbers the step is 2^-24 in those units: an error of up to 2^-25 2^-14 2^e a key, times its code, |code| <= Q.  All
+    keys together: n 2^-39 Q max s, and Q max s is the largest |v| (every row has a code of Q).  Native f16 weights have the
+    same step, with 2^e = 1."""
     d, n = q.shape[-1], max(lens + [1])
-    o, l, spread, size = PO.attention(q, pool, fmt, table, lens, pages, sm_scale)
+    o, l, spread, size, vmax = PO.attention(q, pool, fmt, table, lens, pages, sm_scale)
     out, lse = out.double().cpu(), lse.double().cpu()
-    o, l, spread, size = (t.cpu() for t in (o, l, spread, size))
+    o, l, spread, size, vmax = (t.cpu() for t in (o, l, spread, size, vmax))
     rel = 2.0 ** -11 + 2 * d * 2.0 ** -23 * size + n * 2.0 ** -23
-    tol = torch.finfo(q.dtype).eps / 2 * o.abs() + rel[..., None] * spread + 1e-30
+    tol = torch.finfo(q.dtype).eps / 2 * o.abs() + rel[..., None] * spread + n * 2.0 ** -39 * vmax[..., None]
     tiny = torch.finfo(q.dtype).tiny
     assert ((out - o).abs() <= tol + tiny).all(), ((out - o).abs() / (tol + tiny)).max()
     empty = l == -float("inf")

@@ -32,69 +32,218 @@ __device__ __forceinline__ int held_pages(const PagedSelectParams& p, int b) {
   return static_cast<int>(min(n, static_cast<long long>(p.table.max_pages)));
 }
 
+template <bool BF16>
+__device__ __forceinline__ uint32_t min16x2_nan(uint32_t a, uint32_t b) {
+  uint32_t r;
+  if (BF16) asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  else asm("min.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+template <bool BF16>
+__device__ __forceinline__ uint32_t max16x2_nan(uint32_t a, uint32_t b) {
+  uint32_t r;
+  if (BF16) asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  else asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+
+constexpr int kScorePages = 4;                                   // pages per lane group, loaded ahead of their use
+__host__ __device__ constexpr int score_pages_per_cta(int d) { return 256 / (d / 8) * kScorePages; }
+
+// D / 8 lanes take a page: 8 channels each, of which a 16-byte load brings the minima and another the maxima.  The larger of
+// u min and u max is the product with the bound of u's sign, so a channel costs one DFMA.  Bound by the bounds' bytes: 512 a
+// page and KV head at D = 128.
 template <int D, bool BF16>
 __global__ void __launch_bounds__(256) paged_score_kernel(const __grid_constant__ PagedSelectParams p) {
-  __shared__ double u[D];
+  constexpr int kLanes = D / 8, kPer = score_pages_per_cta(D);
+  __shared__ double u_s[D];
+  griddep_launch();
   const int h = blockIdx.y, b = blockIdx.z;
+  const int held = held_pages(p, b);
+  if (held <= p.budget || static_cast<int>(blockIdx.x) * kPer >= held) return;   // all of them are taken: nothing to score
+  const int grp = threadIdx.x / kLanes, c = threadIdx.x % kLanes;
+  const int first = blockIdx.x * kPer + grp;
+  uint4 lo[kScorePages], hi[kScorePages];
+  int page[kScorePages];
+#pragma unroll
+  for (int j = 0; j < kScorePages; ++j) {
+    const int i = first + j * (256 / kLanes);
+    page[j] = i < held ? page_of(p.table, b, i, p.pool.num_pages) : -1;
+  }
+#pragma unroll
+  for (int j = 0; j < kScorePages; ++j) {
+    lo[j] = hi[j] = make_uint4(0, 0, 0, 0);
+    if (page[j] >= 0) {
+      const uint4* row = reinterpret_cast<const uint4*>(p.pool.k_bounds) + (static_cast<long long>(page[j]) * p.pool.hkv + h) * 2 * kLanes;
+      lo[j] = row[c];
+      hi[j] = row[kLanes + c];
+    }
+  }
   if (threadIdx.x < D) {
     double s = 0.0;
+#pragma unroll 8
     for (int g = 0; g < p.groups; ++g)
       s += static_cast<double>(to_f32<BF16>(*reinterpret_cast<const uint16_t*>(p.q + 2 * (b * p.q_sb + (h * p.groups + g) * p.q_sh + threadIdx.x))));
-    u[threadIdx.x] = s;
+    u_s[threadIdx.x] = s;
   }
   __syncthreads();
-  const int held = held_pages(p, b);
-  for (int i = blockIdx.x * 256 + threadIdx.x; i < p.table.max_pages; i += 256 * gridDim.x) {
-    unsigned long long key = 0ull;
-    if (i < held) {
-      if (i < p.sink_pages || i >= held - p.recent_pages) {
-        key = ~0ull;
-      } else {
-        const int page = page_of(p.table, b, i, p.pool.num_pages);
-        if (page >= 0) {
-          const uint16_t* lo = reinterpret_cast<const uint16_t*>(p.pool.k_bounds) + (static_cast<long long>(page) * p.pool.hkv + h) * 2 * D;
-          double s = 0.0;
-          for (int d = 0; d < D; ++d) {
-            const double a = u[d] * static_cast<double>(to_f32<BF16>(lo[d])), c = u[d] * static_cast<double>(to_f32<BF16>(lo[D + d]));
-            s += (a != a || a > c) ? a : c;
-          }
-          key = ordered_key(s);
-        }
-      }
+  double u[8];
+  uint32_t sign[4];  // which half of a pair takes its maximum
+#pragma unroll
+  for (int i = 0; i < 8; ++i) u[i] = u_s[c * 8 + i];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) sign[i] = (u[2 * i] >= 0.0 ? 0x0000ffffu : 0u) | (u[2 * i + 1] >= 0.0 ? 0xffff0000u : 0u);
+#pragma unroll
+  for (int j = 0; j < kScorePages; ++j) {
+    const uint32_t a[4] = {lo[j].x, lo[j].y, lo[j].z, lo[j].w}, z[4] = {hi[j].x, hi[j].y, hi[j].z, hi[j].w};
+    double s = 0.0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t w = (max16x2_nan<BF16>(a[i], z[i]) & sign[i]) | (min16x2_nan<BF16>(a[i], z[i]) & ~sign[i]);
+      s = fma(u[2 * i], static_cast<double>(to_f32<BF16>(static_cast<uint16_t>(w & 0xffffu))), s);
+      s = fma(u[2 * i + 1], static_cast<double>(to_f32<BF16>(static_cast<uint16_t>(w >> 16))), s);
     }
-    p.keys[(static_cast<long long>(b) * p.pool.hkv + h) * p.table.max_pages + i] = key;
+#pragma unroll
+    for (int o = kLanes / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    const int i = first + j * (256 / kLanes);
+    if (c == 0 && i < held) {
+      unsigned long long key = page[j] >= 0 ? ordered_key(s) : 0ull;
+      if (i < p.sink_pages || i >= held - p.recent_pages) key = ~0ull;
+      p.keys[(static_cast<long long>(b) * p.pool.hkv + h) * p.table.max_pages + i] = key;
+    }
   }
 }
 
-// One CTA per (KV head, sequence): a page is taken if fewer than `budget` come before it; the list is ascending.
+constexpr int kPickBins = 2048;
+
+// exclusive sum over the CTA's 1024 threads in thread order; `total` is everyone's sum.  Ends with a barrier.
+__device__ __forceinline__ int cta_exclusive_sum(int x, int* scratch, int& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int inc = x;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += y;
+  }
+  if (lane == 31) scratch[warp] = inc;
+  __syncthreads();
+  int w = scratch[lane], wi = w;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, wi, o);
+    if (lane >= o) wi += y;
+  }
+  total = __shfl_sync(0xffffffffu, wi, 31);
+  const int before = __shfl_sync(0xffffffffu, wi - w, warp);
+  __syncthreads();
+  return before + inc - x;
+}
+
+// One CTA per (KV head, sequence).  The budget-th highest key is found by histograms: 2048 equal bins over the range of the
+// keys still in question, then over the bin that the budget ends in, until that bin holds no more keys than are wanted or one
+// value only (two rounds for scores as they occur, six at most).  A thread takes 16 consecutive keys at a time, so that one
+// sum over the CTA gives the ascending list; keys are read again in every round, from L1 up to 16384 pages.
 __global__ void __launch_bounds__(1024) paged_pick_kernel(const __grid_constant__ PagedSelectParams p) {
-  __shared__ int base, warp_sum[32];
-  const int h = blockIdx.x, b = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  constexpr int kRun = 16;
+  __shared__ int hist[kPickBins], scratch[32], found[3];
+  __shared__ unsigned long long red[2][32];
+  griddep_launch();
+  griddep_wait();  // the keys come from the kernel launched just before, the lengths from anywhere
+  const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const unsigned long long* keys = p.keys + (static_cast<long long>(b) * p.pool.hkv + h) * p.table.max_pages;
   int* out = p.out + (static_cast<long long>(b) * p.pool.hkv + h) * p.budget;
   const int held = held_pages(p, b);
-  if (threadIdx.x == 0) base = 0;
-  __syncthreads();
-  for (int i0 = 0; i0 < held; i0 += 1024) {
-    const int i = i0 + threadIdx.x;
-    bool take = false;
-    if (i < held) {
-      const unsigned long long mine = keys[i];
-      int before = 0;
-      for (int j = 0; j < held; ++j) before += keys[j] > mine || (keys[j] == mine && j < i);
-      take = before < p.budget;
+  if (held <= p.budget) {
+    for (int i = tid; i < p.budget; i += 1024) out[i] = i < held ? i : -1;
+    return;
+  }
+  // pages that are taken without a score (sink + recent <= budget < held, so the two do not meet)
+  const int lo_i = p.sink_pages, hi_i = held - p.recent_pages;
+  int want = p.budget - p.sink_pages - p.recent_pages;
+  unsigned long long lo = ~0ull, hi = 0ull;
+  for (int i0 = 0; i0 < held; i0 += 1024 * kRun)
+#pragma unroll
+    for (int j = 0; j < kRun; ++j) {
+      const int i = i0 + tid * kRun + j;
+      if (i >= lo_i && i < hi_i) {
+        const unsigned long long k = keys[i];
+        lo = min(lo, k);
+        hi = max(hi, k);
+      }
     }
-    const unsigned votes = __ballot_sync(0xffffffffu, take);
-    if (lane == 0) warp_sum[warp] = __popc(votes);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    lo = min(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+    hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+  }
+  if (lane == 0) { red[0][warp] = lo; red[1][warp] = hi; }
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 32; ++w) { lo = min(lo, red[0][w]); hi = max(hi, red[1][w]); }
+  // keys above `hi` are taken, keys below `lo` are not, `want` of those between are.  (hi < ~0: no score has that key.)
+  unsigned long long from = hi + 1ull;  // what is taken without a look at its place
+  while (want > 0) {
+    const unsigned long long span = hi - lo;
+    const int shift = max(0, 53 - __clzll(span));  // (hi - lo) >> shift < 2048
+    hist[tid] = hist[1024 + tid] = 0;
     __syncthreads();
-    int at = base + __popc(votes & ((1u << lane) - 1u));
-    for (int w = 0; w < warp; ++w) at += warp_sum[w];
-    if (take) out[at] = i;
+    for (int i0 = 0; i0 < held; i0 += 1024 * kRun)
+#pragma unroll
+      for (int j = 0; j < kRun; ++j) {
+        const int i = i0 + tid * kRun + j;
+        if (i >= lo_i && i < hi_i) {
+          const unsigned long long k = keys[i];
+          if (k >= lo && k <= hi) atomicAdd(&hist[static_cast<int>((k - lo) >> shift)], 1);
+        }
+      }
     __syncthreads();
-    if (threadIdx.x == 1023) base = at + take;
+    // from the highest bin down: thread t has bins 2047 - 2 t and 2046 - 2 t
+    const int b0 = kPickBins - 1 - 2 * tid, n0 = hist[b0], n1 = hist[b0 - 1];
+    int total;
+    const int above = cta_exclusive_sum(n0 + n1, scratch, total);
+    if (above < want && above + n0 + n1 >= want) {
+      const bool second = above + n0 < want;
+      found[0] = second ? b0 - 1 : b0;
+      found[1] = second ? above + n0 : above;  // keys in higher bins
+      found[2] = second ? n1 : n0;
+    }
+    __syncthreads();
+    const int bin = found[0], higher = found[1], inside = found[2];
+    want -= higher;
+    const unsigned long long bin_lo = lo + (static_cast<unsigned long long>(bin) << shift);
+    const unsigned long long width = (1ull << shift) - 1ull;
+    const unsigned long long bin_hi = hi - bin_lo < width ? hi : bin_lo + width;
+    lo = bin_lo;
+    hi = bin_hi;
+    from = hi + 1ull;
+    if (inside == want) { from = lo; want = 0; break; }  // all of the bin
+    if (lo == hi) break;                                 // one value: the lowest pages of it
     __syncthreads();
   }
-  for (int i = base + threadIdx.x; i < p.budget; i += 1024) out[i] = -1;
+  int taken = 0, ties = 0;  // before this chunk
+  for (int i0 = 0; i0 < held; i0 += 1024 * kRun) {
+    unsigned take = 0, tie = 0;
+#pragma unroll
+    for (int j = 0; j < kRun; ++j) {
+      const int i = i0 + tid * kRun + j;
+      if (i >= held) continue;
+      const bool always = i < lo_i || i >= hi_i;
+      const unsigned long long k = always ? 0ull : keys[i];
+      if (always || k >= from) take |= 1u << j;
+      else if (want > 0 && k == lo) tie |= 1u << j;
+    }
+    int all;
+    const int tie_at = ties + cta_exclusive_sum(__popc(tie), scratch, all);
+    ties += all;
+    for (int room = want - tie_at; tie && room > 0; --room) {  // the lowest of this thread's ties that there is room for
+      const unsigned low = tie & (0u - tie);
+      take |= low;
+      tie ^= low;
+    }
+    int at = taken + cta_exclusive_sum(__popc(take), scratch, all);
+    taken += all;
+    for (; take; take &= take - 1) out[at++] = i0 + tid * kRun + __ffs(take) - 1;
+  }
 }
 
 }  // namespace sq

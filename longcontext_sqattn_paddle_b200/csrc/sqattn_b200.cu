@@ -1460,11 +1460,15 @@ int sqattn_paged_select(const sqattn_paged_select_args* a, sqattn_stream_t strea
   p.kv_lens = a->kv_lens; p.batch = a->batch; p.groups = a->num_q_heads / a->pool->num_kv_heads;
   p.budget = a->budget; p.sink_pages = a->sink_pages; p.recent_pages = a->recent_pages;
   p.keys = static_cast<unsigned long long*>(a->workspace); p.out = a->out;
-  const dim3 grid((a->max_pages + 255) / 256, a->pool->num_kv_heads, a->batch);
   const bool bf16 = a->pool->dtype == SQATTN_BF16;
-  if (a->pool->head_dim == 128) { if (bf16) paged_score_kernel<128, true><<<grid, 256, 0, stream>>>(p); else paged_score_kernel<128, false><<<grid, 256, 0, stream>>>(p); }
-  else { if (bf16) paged_score_kernel<64, true><<<grid, 256, 0, stream>>>(p); else paged_score_kernel<64, false><<<grid, 256, 0, stream>>>(p); }
-  paged_pick_kernel<<<dim3(a->pool->num_kv_heads, a->batch), 1024, 0, stream>>>(p);
+  if (a->max_pages > a->budget) {   // else every page is taken
+    const int per = score_pages_per_cta(a->pool->head_dim);
+    const dim3 grid((a->max_pages + per - 1) / per, a->pool->num_kv_heads, a->batch);
+    if (a->pool->head_dim == 128) { if (bf16) paged_score_kernel<128, true><<<grid, 256, 0, stream>>>(p); else paged_score_kernel<128, false><<<grid, 256, 0, stream>>>(p); }
+    else { if (bf16) paged_score_kernel<64, true><<<grid, 256, 0, stream>>>(p); else paged_score_kernel<64, false><<<grid, 256, 0, stream>>>(p); }
+    SQ_CUDA(cudaGetLastError());
+  }
+  SQ_CUDA(launch_overlapped(1, paged_pick_kernel, dim3(a->pool->num_kv_heads, a->batch), dim3(1024), 0, stream, p));
   SQ_CUDA(cudaGetLastError());
   return SQATTN_OK;
 }

@@ -2,14 +2,16 @@
 //
 // Memory bound: per key and KV head 2 * row bytes (+ 8 for codes) are read once for all query heads of the group.
 //
-// Work.  A tile is 32 keys of one (sequence, KV head) segment.  All tiles of all segments stand in one row, and every CTA
-// takes an equal stretch of it, whatever the lengths, which the kernel reads itself; so a captured launch stays balanced
-// while the cache grows, and a ragged batch needs no plan.  A segment that lies in one CTA is finished there, one that is
-// cut leaves partial results for paged_merge_kernel.
+// Work.  A tile is 32 or 64 keys of one (sequence, KV head) segment.  All tiles of all segments stand in one row, and every
+// warp of the grid takes an equal stretch of it, whatever the lengths, which the kernel reads itself; so a captured launch
+// stays balanced while the cache grows, and a ragged batch needs no plan.  A segment that lies in one warp's stretch is
+// finished by that warp alone; pieces of a segment that several warps share are joined at the end of the CTA, and what CTAs
+// share by paged_merge_kernel.
 //
-// Copies.  A warp is its own producer: it keeps kStages of its tiles in flight in a ring of its own (TMA boxes of 16 or 32
-// rows, 128-byte swizzle, scales by bulk copies), so that warps never wait for one another between segments, and the ring
-// runs on across segments.  Where a tile's pages lie is looked up by one lane per tile, 32 tiles at a time.
+// Copies.  A warp is its own producer: it keeps kStages of its tiles in flight in a ring of its own (TMA boxes of 16 to 64
+// rows, 128-byte swizzle, scales by bulk copies), so that warps never wait for one another before the end of the CTA, and the
+// ring runs on across segments.  Where a tile's pages lie is looked up by one lane per tile, 32 tiles at a time, and that lane
+// issues the tile's copies.
 //
 // Arithmetic.  S^T = K Q^T and O^T = V^T P^T on mma.sync m16n8k16 with the keys (channels) as rows and the query heads as
 // the 8 columns: with at most 8 heads to a group no product is padding but the unused heads' columns.  The products do not
@@ -29,7 +31,6 @@
 
 namespace sq {
 
-constexpr int kPagedTile = 32;
 constexpr int kPagedMaxBatch = 1024;
 
 struct PagedDecodeParams {
@@ -45,30 +46,33 @@ struct PagedDecodeParams {
   int list_len;
   int max_len;  // what the table, or the caller's bound, holds
   int batch, hq, groups, q_bf16, o_bf16;
-  int min_tiles;     // a CTA takes at least so many
   float scale_log2;  // softmax scale * log2(e)
   float* part_o;     // [grid + B * Hkv, groups, D] fp32, each divided by its own sum
   float* part_lse;   // [grid + B * Hkv, groups]
+  float* piece_o;    // [grid * warps, groups, D] fp32: what a warp's first segment has of it, if that ends inside the stretch
   int* plan;         // [B + 2]: tiles per KV head before each sequence, then tiles per CTA
+  int* cut;          // [grid]: segment that begins in the CTA before and goes on in this one, or -1
 };
 
 template <int FMT, int D, int NT>
 struct PagedDecodeCfg {
   static constexpr int kRow = kv_row_bytes<FMT>(D);
-  static constexpr int kWarps = (FMT == kKvNative && D == 128) ? 4 : 8;
-  static constexpr int kStages = FMT == kKvNative ? (D == 128 && NT == 1 ? 3 : 2) : (FMT == kKvInt8 && D == 128 ? 2 : 4);
-  static constexpr int kTensor = kPagedTile * kRow;                      // a tile's keys or values
-  static constexpr int kRing = kWarps * kStages * 2 * kTensor;
-  static constexpr int kScaleOff = kRing;                                // [warp][stage][K, V][32] fp32
-  static constexpr int kScales = FMT == kKvNative ? 0 : kWarps * kStages * 256;
-  static constexpr int kRedOff = kScaleOff + kScales;                    // [warp][8 NT][D] fp32
-  static constexpr int kMlOff = kRedOff + kWarps * 8 * NT * D * 4;       // [warp][8 NT] maxima, then sums
-  static constexpr int kBarOff = kMlOff + kWarps * 8 * NT * 8;           // [warp][stage]
+  static constexpr int kTile = FMT == kKvInt4 ? 64 : 32;                 // keys of a tile
+  static constexpr int kWarps = FMT == kKvNative ? (D == 128 ? 4 : 8) : (NT == 2 ? 8 : 12);
+  static constexpr int kStages = FMT == kKvNative ? 3 : 2;
+  static constexpr int kTensor = kTile * kRow;                           // a tile's keys or values
+  static constexpr int kRingWarp = kStages * 2 * kTensor;
+  static constexpr int kScaleOff = kWarps * kRingWarp;                   // [warp][stage][K, V][kTile] fp32
+  static constexpr int kScaleStage = FMT == kKvNative ? 0 : 2 * kTile * 4;
+  static constexpr int kMlOff = kScaleOff + kWarps * kStages * kScaleStage;  // [2 warps][8 NT] maxima, then sums
+  static constexpr int kBarOff = kMlOff + 2 * kWarps * 8 * NT * 8;       // [warp][stage]
   static constexpr int kInfoOff = kBarOff + kWarps * kStages * 8;        // [warp][stage] valid keys
-  static constexpr int kMiscOff = kInfoOff + kWarps * kStages * 4;       // abort flag
+  static constexpr int kSegOff = kInfoOff + kWarps * kStages * 4;        // [2 warps] segments of the pieces
+  static constexpr int kMiscOff = kSegOff + 2 * kWarps * 4;              // abort flag
   static constexpr int kPlanOff = (kMiscOff + 16 + 15) / 16 * 16;        // [B + 1]
   static constexpr int total(int batch) { return kPlanOff + (batch + 1) * 4 + 1024; }
   static_assert(total(kPagedMaxBatch) <= 227 * 1024, "shared memory of a CTA");
+  static_assert(8 * NT * D * 4 <= kRingWarp, "a warp's last piece takes the place of its ring");
 };
 
 // untiled copy global -> shared, completion counted in bytes on `bar`
@@ -116,10 +120,11 @@ __device__ __forceinline__ uint32_t swizzle128(uint32_t o) { return o ^ ((o >> 3
 
 // tiles of one (sequence, KV head) segment
 __device__ __forceinline__ int paged_len(const PagedDecodeParams& p, int b) { return min(max(p.kv_lens[b], 0), p.max_len); }
+template <int TILE>
 __device__ __forceinline__ int paged_tiles(const PagedDecodeParams& p, int len) {
   if (len == 0) return 0;
-  const long long keys = p.list ? static_cast<long long>(p.list_len) << p.pool.ps_shift : len;
-  return static_cast<int>((keys + kPagedTile - 1) / kPagedTile);
+  const int keys = p.list ? p.list_len << p.pool.ps_shift : len;
+  return static_cast<int>((static_cast<unsigned>(keys) + TILE - 1) / TILE);
 }
 
 template <int FMT, int D, bool BF16, int NT>
@@ -127,8 +132,9 @@ __global__ void __launch_bounds__(PagedDecodeCfg<FMT, D, NT>::kWarps * 32, 1)
 paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                     const __grid_constant__ PagedDecodeParams p) {
   using C = PagedDecodeCfg<FMT, D, NT>;
-  constexpr int W = C::kWarps, S = C::kStages, ROW = C::kRow, NTHR = W * 32, H = 8 * NT;
+  constexpr int W = C::kWarps, S = C::kStages, ROW = C::kRow, TILE = C::kTile, MT = TILE / 16, NTHR = W * 32, H = 8 * NT;
   constexpr bool kNative = FMT == kKvNative;
+  constexpr uint32_t kAllValid = MT == 2 ? 0x1010u : 0x10101010u;
   griddep_launch();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int hkv = p.pool.hkv;
@@ -151,17 +157,17 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
   const uint32_t sbase = smem_u32(smem);
   volatile int* cta_abort = reinterpret_cast<volatile int*>(smem + C::kMiscOff);
   int* pre = reinterpret_cast<int*>(smem + C::kPlanOff);
-  float* red = reinterpret_cast<float*>(smem + C::kRedOff);
-  float* ml = reinterpret_cast<float*>(smem + C::kMlOff);
+  int* seg_of = reinterpret_cast<int*>(smem + C::kSegOff);   // [warp][piece of the first segment, piece of the last]
+  float* ml = reinterpret_cast<float*>(smem + C::kMlOff);    // their maxima [2 W][H], then sums [2 W][H]
   const uint32_t bars = sbase + C::kBarOff + warp * S * 8;
-  volatile int* info = reinterpret_cast<volatile int*>(smem + C::kInfoOff) + warp * S;
+  volatile uint32_t* info = reinterpret_cast<volatile uint32_t*>(smem + C::kInfoOff) + warp * S;
 
   // ---- plan: tiles (of one KV head) before each sequence
   if (warp == 0) {
     int run = 0;
     for (int b0 = 0; b0 < p.batch; b0 += 32) {
       const int b = b0 + lane;
-      const int mine = b < p.batch ? paged_tiles(p, paged_len(p, b)) : 0;
+      const int mine = b < p.batch ? paged_tiles<TILE>(p, paged_len(p, b)) : 0;
       int x = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -172,19 +178,43 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
       run += __shfl_sync(0xffffffffu, x, 31);
     }
     if (lane == 0) pre[p.batch] = run;
-  } else if (warp == 1 && lane == 0) {
-    *cta_abort = 0;
-    for (int i = 0; i < W * S; ++i) mbar_init(sbase + C::kBarOff + 8 * i, 1);
-    fence_barrier_init();
-    fence_proxy_async();
+  } else if (warp == 1) {
+    if (lane < 2 * W) seg_of[lane] = -1;
+    if (lane == 0) {
+      *cta_abort = 0;
+      for (int i = 0; i < W * S; ++i) mbar_init(sbase + C::kBarOff + 8 * i, 1);
+      fence_barrier_init();
+      fence_proxy_async();
+    }
   }
   __syncthreads();
-  const long long total = static_cast<long long>(pre[p.batch]) * hkv;
-  const long long share = (total + gridDim.x - 1) / gridDim.x;
-  const int per = static_cast<int>(share > p.min_tiles ? share : p.min_tiles);
+  // the host has checked that all tiles of a call fit 31 bits
+  const int total = pre[p.batch] * hkv;
+  const int per = max((total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x), W);
+  const long long cta_first = static_cast<long long>(blockIdx.x) * per;
+  const int x0 = static_cast<int>(min(cta_first, static_cast<long long>(total)));
+  const int x1 = static_cast<int>(min(cta_first + per, static_cast<long long>(total)));
+
+  // sequence of tile x
+  auto seq_of = [&](int x) {
+    int lo = 0, hi = p.batch;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (pre[mid] * hkv <= x) lo = mid; else hi = mid;
+    }
+    return lo;
+  };
   if (blockIdx.x == 0) {
     for (int b = tid; b <= p.batch; b += NTHR) p.plan[b] = pre[b];
     if (tid == 0) p.plan[p.batch + 1] = per;
+  }
+  if (tid == 0) {
+    int cut = -1;
+    if (x0 > 0 && x0 < x1) {
+      const int b = seq_of(x0), n = pre[b + 1] - pre[b], h = (x0 - pre[b] * hkv) / n, first = pre[b] * hkv + h * n;
+      if (first < x0 && first / per == static_cast<int>(blockIdx.x) - 1) cut = b * hkv + h;
+    }
+    p.cut[blockIdx.x] = cut;
   }
   // sequences without keys: zeros
   for (int b = blockIdx.x; b < p.batch; b += gridDim.x)
@@ -193,105 +223,88 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         store_o(b, i / D, i % D, 0.0f);
         if (p.lse && i % D == 0) p.lse[static_cast<long long>(b) * p.hq + i / D] = -INFINITY;
       }
-  const long long x0 = static_cast<long long>(blockIdx.x) * per;
-  const long long x1 = min(total, x0 + per);
   if (x0 >= x1) return;
+  const int share = (x1 - x0 + W - 1) / W;
+  const int xw0 = min(x1, x0 + warp * share), xw1 = min(x1, xw0 + share);   // this warp's stretch
 
-  // sequence of tile x
-  auto seq_of = [&](long long x) {
-    int lo = 0, hi = p.batch;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (static_cast<long long>(pre[mid]) * hkv <= x) lo = mid; else hi = mid;
-    }
-    return lo;
-  };
-
-  // ---- copies.  Lane i looks up the i-th of the warp's next 32 tiles: rec_ph page * Hkv + head of its (one or two) pages,
-  // rec_row the first row inside the page, rec_nv the valid keys of its first and second half
+  // ---- copies.  Lane i looks up the i-th of the warp's next 32 tiles: for each 16 keys of it page * Hkv + head and the number of
+  // valid ones (8 bits each), and the first row inside the page (pages of fewer rows than a tile begin at their row 0)
   const int ps = 1 << p.pool.ps_shift;
-  const uint32_t ring = sbase + warp * (S * 2 * C::kTensor);
-  const uint32_t scales = sbase + C::kScaleOff + warp * S * 256;
-  int rec_ph[2], rec_row = 0, rec_nv = 0;
-  auto look_up = [&](long long x) {
-    rec_ph[0] = rec_ph[1] = 0;
-    rec_row = rec_nv = 0;
-    if (x >= x1) return;
-    const int b = seq_of(x);
-    const int n = pre[b + 1] - pre[b];
-    const long long rem = x - static_cast<long long>(pre[b]) * hkv;
-    const int h = static_cast<int>(rem / n);
-    const int key = static_cast<int>(rem % n) * kPagedTile;
-    const int len = paged_len(p, b);
-    const int held = static_cast<int>((static_cast<long long>(len) + ps - 1) >> p.pool.ps_shift);
-    rec_row = key & (ps - 1);
+  const uint32_t ring = sbase + warp * C::kRingWarp;
+  const uint32_t scales = sbase + C::kScaleOff + warp * S * C::kScaleStage;
+  const int box = kNative ? 16 : min(ps, TILE);   // rows of a copy, as the tensor maps have it
+  int rec_ph[MT], rec_row = 0;
+  uint32_t rec_nv = 0;
+  auto look_up = [&](int x) {
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {   // the tile's halves lie in one page unless pages have 16 rows
-      const int at = (key + 16 * s) >> p.pool.ps_shift;
-      int index = at;
-      if (p.list) index = at < p.list_len ? p.list[(static_cast<long long>(b) * hkv + h) * p.list_len + at] : -1;
-      if (index < 0 || index >= held) continue;
-      const int page = page_of(p.table, b, index, p.pool.num_pages);
-      if (page < 0) continue;
-      rec_ph[s] = page * hkv + h;
-      const long long left = len - ((static_cast<long long>(index) << p.pool.ps_shift) + ((key + 16 * s) & (ps - 1)));
-      rec_nv |= static_cast<int>(min(max(left, 0ll), 16ll)) << (8 * s);
+    for (int s = 0; s < MT; ++s) rec_ph[s] = 0;
+    rec_row = 0;
+    rec_nv = 0;
+    if (x >= xw1) return;
+    const int b = seq_of(x);
+    const int n = pre[b + 1] - pre[b], rem = x - pre[b] * hkv;
+    const int h = rem / n, key = (rem - h * n) * TILE;
+    const int len = paged_len(p, b);
+    const int held = static_cast<int>((static_cast<unsigned>(len) + ps - 1) >> p.pool.ps_shift);
+    rec_row = key & (ps - 1);
+    int at_last = -1, ph = 0, first = 0;
+#pragma unroll
+    for (int s = 0; s < MT; ++s) {
+      const int at = static_cast<int>(static_cast<unsigned>(key + 16 * s) >> p.pool.ps_shift);
+      if (at != at_last) {
+        at_last = at;
+        int index = at;
+        if (p.list) index = at < p.list_len ? p.list[(static_cast<long long>(b) * hkv + h) * p.list_len + at] : -1;
+        const int page = index >= 0 && index < held ? page_of(p.table, b, index, p.pool.num_pages) : -1;
+        ph = page * hkv + h;
+        first = page >= 0 ? index << p.pool.ps_shift : len;   // position of the page's row 0
+      }
+      rec_ph[s] = ph;
+      const int left = len - first - ((key + 16 * s) & (ps - 1));
+      rec_nv |= static_cast<uint32_t>(min(max(left, 0), 16)) << (8 * s);
     }
   };
-  long long xi = x0 + warp;  // next tile to copy
-  int ahead = 32;            // place of that tile among the looked-up ones
+  int xi = xw0, ahead = 32;  // next tile to copy, its place among the looked-up ones
   auto issue = [&](int st) {
-    if (xi >= x1) return;
+    if (xi >= xw1) return;
     if (ahead == 32) {
-      look_up(xi + static_cast<long long>(lane) * W);
+      look_up(xi + lane);
       ahead = 0;
     }
-    const int ph0 = __shfl_sync(0xffffffffu, rec_ph[0], ahead), ph1 = __shfl_sync(0xffffffffu, rec_ph[1], ahead);
-    const int row = __shfl_sync(0xffffffffu, rec_row, ahead), nv = __shfl_sync(0xffffffffu, rec_nv, ahead);
-    ++ahead;
-    xi += W;
-    if (lane == 0) {
-      info[st] = nv;
-      const uint32_t bar = bars + 8 * st, dst = ring + st * (2 * C::kTensor), sdst = scales + st * 256;
-      const bool a = (nv & 0xff) != 0, b = (nv >> 8) != 0;
-      if (kNative || p.pool.ps_shift == 4) {
-        // boxes of 16 rows
-        constexpr int kBox = 16 * ROW, kBlk = kNative ? 16 : 16 * ROW / 128;
-        constexpr uint32_t kBytes = 2 * kBox + (kNative ? 0 : 128);
-        mbar_expect_tx(bar, (a ? kBytes : 0u) + (b ? kBytes : 0u));
-        const int row1 = p.pool.ps_shift == 4 ? 0 : row + 16;
+    if (lane == ahead) {
+      info[st] = rec_nv;
+      const uint32_t bar = bars + 8 * st, dst = ring + st * (2 * C::kTensor), sdst = scales + st * C::kScaleStage;
+      const int step = box >> 4;   // in units of 16 rows
+      // valid rows come first in a page, so a box has some if its first 16 have
+      int boxes = 0;
 #pragma unroll
-        for (int s = 0; s < 2; ++s)
-          if (s ? b : a) {
-            const int ph = s ? ph1 : ph0, r = s ? row1 : row;
-            tma_load_4d(dst + s * kBox, &tm_k, bar, 0, r / 16 * kBlk, 0, ph);
-            tma_load_4d(dst + C::kTensor + s * kBox, &tm_v, bar, 0, r / 16 * kBlk, 0, ph);
-            if (!kNative) {
-              const long long off = (static_cast<long long>(ph) << p.pool.ps_shift) + r;
-              bulk_load(sdst + s * 64, p.pool.k_scale + off, 64, bar);
-              bulk_load(sdst + 128 + s * 64, p.pool.v_scale + off, 64, bar);
-            }
+      for (int s = 0; s < MT; ++s) boxes += (s & (step - 1)) == 0 && ((rec_nv >> (8 * s)) & 0xffu) != 0u;
+      mbar_expect_tx(bar, boxes * box * (2 * ROW + (kNative ? 0 : 8)));
+#pragma unroll
+      for (int s = 0; s < MT; ++s)
+        if ((s & (step - 1)) == 0 && ((rec_nv >> (8 * s)) & 0xffu) != 0u) {
+          const int row = (rec_row + 16 * s) & (ps - 1);
+          const int line = kNative ? row : row * ROW / 128;
+          tma_load_4d(dst + s * (16 * ROW), &tm_k, bar, 0, line, 0, rec_ph[s]);
+          tma_load_4d(dst + C::kTensor + s * (16 * ROW), &tm_v, bar, 0, line, 0, rec_ph[s]);
+          if (!kNative) {
+            const long long off = (static_cast<long long>(rec_ph[s]) << p.pool.ps_shift) + row;
+            bulk_load(sdst + s * 64, p.pool.k_scale + off, box * 4, bar);
+            bulk_load(sdst + (TILE + s * 16) * 4, p.pool.v_scale + off, box * 4, bar);
           }
-      } else {
-        // one box of 32 rows
-        mbar_expect_tx(bar, a ? 2u * C::kTensor + 256u : 0u);
-        if (a) {
-          tma_load_4d(dst, &tm_k, bar, 0, row / 32 * (32 * ROW / 128), 0, ph0);
-          tma_load_4d(dst + C::kTensor, &tm_v, bar, 0, row / 32 * (32 * ROW / 128), 0, ph0);
-          const long long off = (static_cast<long long>(ph0) << p.pool.ps_shift) + row;
-          bulk_load(sdst, p.pool.k_scale + off, 128, bar);
-          bulk_load(sdst + 128, p.pool.v_scale + off, 128, bar);
         }
-      }
     }
+    ++ahead;
+    ++xi;
     __syncwarp();
   };
 #pragma unroll 1
   for (int st = 0; st < S; ++st) issue(st);
 
-  // ---- where this lane's pieces of a tile lie
-  uint32_t koff[2][2][2], voff[2][4];  // codes: [half of the tile][rows 0-7, 8-15][piece], [half][rows 2t, 2t+1, 2t+8, 2t+9]
-  uint32_t kx[4], vx[4];               // native: 16-byte chunks (by ldmatrix lane) of channels 16 i .. 16 i + 15 within 64
+  // ---- where this lane's pieces of a tile lie.  The swizzle repeats every 1024 bytes, so these are the places that differ
+  // by less; codes: keys [rows 0-7 or 8-15][piece], values [rows 2t, 2t+1, 2t+8, 2t+9]; native: 16-byte chunks by ldmatrix
+  // lane of channels 16 i .. 16 i + 15 within 64
+  uint32_t kx[4], vx[8];
   if (kNative) {
     const int kr = (lane & 7) + ((lane >> 3) & 1) * 8, kc = lane >> 4;
     const int vr = (lane & 7) + (lane >> 4) * 8, vc = (lane >> 3) & 1;
@@ -301,34 +314,41 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
       vx[i] = C::kTensor + vr * 128 + (((2 * i + vc) ^ (vr & 7)) << 4);
     }
   } else {
-    constexpr int kPiece = ROW == 32 ? 8 : 16, kPieces = ROW == 128 ? 2 : 1;  // keys: ROW / 4 bytes a lane; values: ROW / 8
 #pragma unroll
-    for (int mt = 0; mt < 2; ++mt) {
-#pragma unroll
-      for (int hi = 0; hi < 2; ++hi)
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-          koff[mt][hi][j] = swizzle128((mt * 16 + hi * 8 + row_perm<ROW>(g)) * ROW + (t * kPieces + (j < kPieces ? j : 0)) * kPiece);
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        voff[mt][i] = C::kTensor + swizzle128((mt * 16 + (i >> 1) * 8 + row_perm<ROW>(2 * t + (i & 1))) * ROW + g * (ROW / 8));
+    for (int i = 0; i < 4; ++i) {
+      // ROW 128: i = piece;  64: i = rows 0-7 / 8-15;  32: i = rows 0-7, 8-15, 16-23, 24-31
+      const int row = ROW == 128 ? 0 : 8 * i, piece = ROW == 128 ? 2 * t + (i & 1) : t;
+      kx[i] = swizzle128((row + row_perm<ROW>(g)) * ROW + piece * (ROW == 32 ? 8 : 16));
     }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      vx[i] = C::kTensor + swizzle128(((i >> 1) * 8 + row_perm<ROW>(2 * t + (i & 1))) * ROW + g * (ROW / 8));
   }
-  const int key_row = kNative ? g : row_perm<ROW>(g);  // this lane's first key in a half: that row and the one 8 further
+  // offsets of 16 keys' pieces from those
+  auto k_off = [&](int mt, int hi, int j) -> uint32_t {
+    if (ROW == 128) return kx[j] + (mt * 2 + hi) * 1024;
+    if (ROW == 64) return kx[hi] + mt * 1024;
+    return kx[(mt & 1) * 2 + hi] + (mt >> 1) * 1024;
+  };
+  auto v_off = [&](int mt, int i) -> uint32_t {
+    if (ROW == 128) return vx[i & 1] + (mt * 2 + (i >> 1)) * 1024;
+    if (ROW == 64) return vx[i] + mt * 1024;
+    return vx[(mt & 1) * 4 + i] + (mt >> 1) * 1024;
+  };
+  const int key_row = kNative ? g : row_perm<ROW>(g);  // this lane's first key of 16: that row and the one 8 further
 
   int st = 0;
   uint32_t parity = 0;
   bool ok = true;
-  long long xc = x0 + warp;
-  int b = seq_of(x0);
-  for (long long seg_x = x0; seg_x < x1;) {
-    // ---- segment (b, h): tiles [seg_x, seg_end) of it are this CTA's
-    while (static_cast<long long>(pre[b + 1]) * hkv <= seg_x) ++b;
-    const int n = pre[b + 1] - pre[b];
-    const long long b_start = static_cast<long long>(pre[b]) * hkv;
-    const int h = static_cast<int>((seg_x - b_start) / n);
-    const long long seg_first = b_start + static_cast<long long>(h) * n, seg_last = seg_first + n;
-    const long long seg_end = min(seg_last, x1);
+  int xc = xw0;
+  int b = seq_of(min(xw0, total - 1));
+  while (xc < xw1) {
+    // ---- segment (b, h): tiles [xc, seg_end) of it are this warp's
+    while (pre[b + 1] * hkv <= xc) ++b;
+    const int n = pre[b + 1] - pre[b], b_start = pre[b] * hkv;
+    const int h = (xc - b_start) / n;
+    const int seg_first = b_start + h * n, seg_last = seg_first + n, seg_end = min(seg_last, xw1);
+    const bool whole = seg_first >= xw0 && seg_last <= xw1;
 
     // ---- query heads as the products' 8 columns
     uint32_t qb[NT][D / 16][2];
@@ -387,19 +407,18 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
       for (int i = 0; i < D / 16; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.0f;
     }
     uint32_t vexp = 27u << 23;  // exponent of the largest value scale so far
-    const bool any_tile = xc < seg_end;
 
-    for (; ok && xc < seg_end; xc += W) {
-      ok = mbar_wait_warp(bars + 8 * st, parity, cta_abort, 401);
+    for (; xc < seg_end; ++xc) {
+      ok = ok && mbar_wait_warp(bars + 8 * st, parity, cta_abort, 401);
       if (!ok) break;
-      const int nv = info[st];
+      const uint32_t nv = info[st];
       const uint32_t tile = ring + st * (2 * C::kTensor);
       if (nv != 0) {
-        if (kNative && nv != 0x1010) {
+        if (kNative && nv != kAllValid) {
           // rows behind the sequence (or of a page that is not there) may hold anything: zeros, so that 0 * x is 0
-          for (int i = lane; i < 32 * (ROW / 16); i += 32) {
+          for (int i = lane; i < TILE * (ROW / 16); i += 32) {
             const int r = i / (ROW / 16), c = i % (ROW / 16);
-            if ((r & 15) >= ((nv >> (8 * (r >> 4))) & 0xff))
+            if ((r & 15) >= static_cast<int>((nv >> (8 * (r >> 4))) & 0xffu))
               *reinterpret_cast<uint4*>(smem + (tile - sbase) + C::kTensor + (r >> 4) * (16 * ROW) + (c >> 3) * 2048 + (r & 15) * 128 + (c & 7) * 16) =
                   make_uint4(0, 0, 0, 0);
           }
@@ -407,17 +426,17 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
           __syncwarp();
         }
         // ---- scores
-        float s[NT][2][4];
+        float s[NT][MT][4];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int mt = 0; mt < 2; ++mt) s[nt][mt][0] = s[nt][mt][1] = s[nt][mt][2] = s[nt][mt][3] = 0.0f;
-        float vs[2][2];  // value scales of this lane's keys
+          for (int mt = 0; mt < MT; ++mt) s[nt][mt][0] = s[nt][mt][1] = s[nt][mt][2] = s[nt][mt][3] = 0.0f;
+        float vs[MT][2];  // value scales of this lane's keys
         if (kNative) {
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk)
 #pragma unroll
-            for (int mt = 0; mt < 2; ++mt) {
+            for (int mt = 0; mt < MT; ++mt) {
               uint32_t a[4];
               ldmatrix_x4(tile + kx[kk & 3] + mt * (16 * ROW) + (kk >> 2) * 2048, a[0], a[1], a[2], a[3]);
 #pragma unroll
@@ -426,7 +445,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         } else {
           const uint8_t* tp = smem + (tile - sbase);
 #pragma unroll
-          for (int mt = 0; mt < 2; ++mt) {
+          for (int mt = 0; mt < MT; ++mt) {
             constexpr int kWords = ROW / 16;  // 4-byte words of a key per lane
             uint32_t w[2][kWords];
 #pragma unroll
@@ -434,10 +453,10 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
 #pragma unroll
               for (int j = 0; j < (kWords + 3) / 4; ++j) {
                 if (kWords == 2) {
-                  const uint2 v = *reinterpret_cast<const uint2*>(tp + koff[mt][hi][0]);
+                  const uint2 v = *reinterpret_cast<const uint2*>(tp + k_off(mt, hi, 0));
                   w[hi][0] = v.x; w[hi][1] = v.y;
                 } else {
-                  const uint4 v = *reinterpret_cast<const uint4*>(tp + koff[mt][hi][j]);
+                  const uint4 v = *reinterpret_cast<const uint4*>(tp + k_off(mt, hi, j));
                   w[hi][4 * j] = v.x; w[hi][4 * j + 1] = v.y; w[hi][4 * j + 2] = v.z; w[hi][4 * j + 3] = v.w;
                 }
               }
@@ -462,23 +481,23 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
             }
           }
           // scales
-          const float* sc = reinterpret_cast<const float*>(smem + C::kScaleOff + (warp * S + st) * 256);
+          const float* sc = reinterpret_cast<const float*>(smem + (scales - sbase) + st * C::kScaleStage);
 #pragma unroll
-          for (int mt = 0; mt < 2; ++mt)
+          for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
             for (int hi = 0; hi < 2; ++hi) {
               const float ks = sc[mt * 16 + hi * 8 + key_row];
-              vs[mt][hi] = sc[32 + mt * 16 + hi * 8 + key_row];
+              vs[mt][hi] = sc[TILE + mt * 16 + hi * 8 + key_row];
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt) { s[nt][mt][2 * hi] *= ks; s[nt][mt][2 * hi + 1] *= ks; }
             }
         }
-        if (nv != 0x1010) {
+        if (nv != kAllValid) {
 #pragma unroll
-          for (int mt = 0; mt < 2; ++mt)
+          for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
             for (int hi = 0; hi < 2; ++hi)
-              if (hi * 8 + key_row >= ((nv >> (8 * mt)) & 0xff)) {
+              if (hi * 8 + key_row >= static_cast<int>((nv >> (8 * mt)) & 0xffu)) {
                 vs[mt][hi] = 0.0f;
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) s[nt][mt][2 * hi] = s[nt][mt][2 * hi + 1] = -INFINITY;
@@ -491,7 +510,9 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            float x = fmaxf(fmaxf(s[nt][0][c], s[nt][0][c + 2]), fmaxf(s[nt][1][c], s[nt][1][c + 2]));
+            float x = fmaxf(s[nt][0][c], s[nt][0][c + 2]);
+#pragma unroll
+            for (int mt = 1; mt < MT; ++mt) x = max3(x, s[nt][mt][c], s[nt][mt][c + 2]);
             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
@@ -500,8 +521,10 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
           }
         uint32_t vexp_new = vexp;
         if (!kNative) {
-          const uint32_t top = __float_as_uint(fmaxf(fmaxf(vs[0][0], vs[0][1]), fmaxf(vs[1][0], vs[1][1])));
-          vexp_new = max(vexp, __reduce_max_sync(0xffffffffu, top) & 0x7f800000u);
+          float top = fmaxf(vs[0][0], vs[0][1]);
+#pragma unroll
+          for (int mt = 1; mt < MT; ++mt) top = max3(top, vs[mt][0], vs[mt][1]);
+          vexp_new = max(vexp, __reduce_max_sync(0xffffffffu, __float_as_uint(top)) & 0x7f800000u);
         }
         if (__any_sync(0xffffffffu, moved) || vexp_new != vexp) {
           // 2^(old - new) of the value scales' exponents
@@ -525,19 +548,23 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
           }
         }
         // ---- weights, 2^14 high, and their two 16-bit parts (native) or products with the value scales (codes)
-        uint32_t pb[NT][2][2], pl[NT][2][2];
+        uint32_t pb[NT][MT][2], pl[NT][MT][2];
+        const float inv = __uint_as_float((254u << 23) - vexp);
+        if (!kNative) {
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) { vs[mt][0] *= inv; vs[mt][1] *= inv; }
+        }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           float off[2];
 #pragma unroll
           for (int c = 0; c < 2; ++c) off[c] = 14.0f - (m[nt][c] == -INFINITY ? 0.0f : m[nt][c] * cs[nt][c]);
-          const float inv = __uint_as_float((254u << 23) - vexp);
 #pragma unroll
-          for (int mt = 0; mt < 2; ++mt)
+          for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
             for (int hi = 0; hi < 2; ++hi) {
-              float w0 = ex2_approx(fmaf(s[nt][mt][2 * hi], cs[nt][0], off[0]));
-              float w1 = ex2_approx(fmaf(s[nt][mt][2 * hi + 1], cs[nt][1], off[1]));
+              const float w0 = ex2_approx(fmaf(s[nt][mt][2 * hi], cs[nt][0], off[0]));
+              const float w1 = ex2_approx(fmaf(s[nt][mt][2 * hi + 1], cs[nt][1], off[1]));
               l[nt][0] += w0;
               l[nt][1] += w1;
               if (kNative) {
@@ -546,15 +573,14 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
                 pb[nt][mt][hi] = movmatrix_trans(head);
                 pl[nt][mt][hi] = movmatrix_trans(BF16 ? pack_bf16x2(w0 - h0, w1 - h1) : pack_f16x2(w0 - h0, w1 - h1));
               } else {
-                const float f = vs[mt][hi] * inv;
-                pb[nt][mt][hi] = movmatrix_trans(pack_f16x2(w0 * f, w1 * f));
+                pb[nt][mt][hi] = movmatrix_trans(pack_f16x2(w0 * vs[mt][hi], w1 * vs[mt][hi]));
               }
             }
         }
         // ---- values
         if (kNative) {
 #pragma unroll
-          for (int mt = 0; mt < 2; ++mt)
+          for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
             for (int i = 0; i < D / 16; ++i) {
               uint32_t a[4];
@@ -568,19 +594,19 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         } else {
           const uint8_t* tp = smem + (tile - sbase);
 #pragma unroll
-          for (int mt = 0; mt < 2; ++mt) {
+          for (int mt = 0; mt < MT; ++mt) {
             constexpr int kWords = ROW / 32;
             uint32_t w[4][kWords];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               if (kWords == 4) {
-                const uint4 v = *reinterpret_cast<const uint4*>(tp + voff[mt][i]);
+                const uint4 v = *reinterpret_cast<const uint4*>(tp + v_off(mt, i));
                 w[i][0] = v.x; w[i][1 % kWords] = v.y; w[i][2 % kWords] = v.z; w[i][3 % kWords] = v.w;
               } else if (kWords == 2) {
-                const uint2 v = *reinterpret_cast<const uint2*>(tp + voff[mt][i]);
+                const uint2 v = *reinterpret_cast<const uint2*>(tp + v_off(mt, i));
                 w[i][0] = v.x; w[i][1 % kWords] = v.y;
               } else {
-                w[i][0] = *reinterpret_cast<const uint32_t*>(tp + voff[mt][i]);
+                w[i][0] = *reinterpret_cast<const uint32_t*>(tp + v_off(mt, i));
               }
             }
 #pragma unroll
@@ -614,93 +640,172 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
       issue(st);
       if (++st == S) { st = 0; parity ^= 1; }
     }
+    xc = ok ? seg_end : xc;
 
-    // ---- the warps' results of this segment: sums over the lanes of a column, then through shared memory
-    __syncthreads();  // everyone is done reading the previous segment's
+    // ---- this warp's result of the segment
+    const float nan = __int_as_float(0x7fc00000);
+    const float unit = kNative ? 1.0f : __uint_as_float(vexp);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
 #pragma unroll
         for (int sh = 4; sh < 32; sh <<= 1) l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], sh);
-        if (g == 0) {
-          const int col = nt * 8 + 2 * t + c;
-          ml[warp * H + col] = m[nt][c] == -INFINITY ? -INFINITY : m[nt][c] * cs[nt][c];
-          ml[(W + warp) * H + col] = l[nt][c];
-        }
+        if (!ok) l[nt][c] = nan;
+        m[nt][c] = m[nt][c] == -INFINITY ? -INFINITY : m[nt][c] * cs[nt][c];  // a NaN sum has no maximum of its own
       }
-    if (any_tile) {
-      const float unit = kNative ? 1.0f : __uint_as_float(vexp);
+    // channel of o[nt][i][e]; e & 1 is the column
+    auto channel = [&](int i, int e) { return kNative ? 16 * i + g + 8 * (e >> 1) : (D / 8) * g + 2 * i + (e >> 1); };
+    if (whole) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int i = 0; i < D / 16; ++i)
+        for (int c = 0; c < 2; ++c) {
+          const int col = nt * 8 + 2 * t + c;
+          if (col < p.groups) {
+            const float f = l[nt][c] != 0.0f ? unit / l[nt][c] : 0.0f;
+            uint16_t* row = reinterpret_cast<uint16_t*>(p.o) + b * p.o_sb + static_cast<long long>(h * p.groups + col) * p.o_sh;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int d = kNative ? 16 * i + g + 8 * (e >> 1) : (D / 8) * g + 2 * i + (e >> 1);
-            red[(warp * H + nt * 8 + 2 * t + (e & 1)) * D + d] = o[nt][i][e] * unit;
+            for (int i = 0; i < D / 16; ++i) {
+              const float a = o[nt][i][c] * f, z = o[nt][i][c + 2] * f;
+              const uint32_t two = p.o_bf16 ? pack_bf16x2(a, z) : pack_f16x2(a, z);
+              if (kNative) {
+                row[channel(i, 0)] = static_cast<uint16_t>(two & 0xffffu);
+                row[channel(i, 2)] = static_cast<uint16_t>(two >> 16);
+              } else {
+                *reinterpret_cast<uint32_t*>(row + channel(i, 0)) = two;
+              }
+            }
+            if (p.lse && g == 0)
+              p.lse[static_cast<long long>(b) * p.hq + h * p.groups + col] =
+                  l[nt][c] != 0.0f ? log2f(l[nt][c]) - 14.0f + (m[nt][c] == -INFINITY ? 0.0f : m[nt][c]) : -INFINITY;
           }
+        }
+    } else {
+      // a piece: the last one of the stretch into the ring, which is empty by then, one before it to global scratch
+      const bool last = seg_end == xw1 || !ok;
+      const int slot = warp * 2 + (last ? 1 : 0);
+      float* to = last ? reinterpret_cast<float*>(smem + warp * C::kRingWarp)
+                       : p.piece_o + (static_cast<long long>(blockIdx.x) * W + warp) * p.groups * D;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const int col = nt * 8 + 2 * t + c;
+          if (col < p.groups) {
+            if (ok) {
+#pragma unroll
+              for (int i = 0; i < D / 16; ++i) {
+                to[col * D + channel(i, 0)] = o[nt][i][c] * unit;
+                to[col * D + channel(i, 2)] = o[nt][i][c + 2] * unit;
+              }
+            }
+            if (g == 0) {
+              ml[slot * H + col] = m[nt][c];
+              ml[(2 * W + slot) * H + col] = l[nt][c];
+            }
+          }
+        }
+      if (lane == 0) seg_of[slot] = b * hkv + h;
     }
-    __syncthreads();
-    const bool whole = seg_first >= x0 && seg_last <= x1;
-    const long long part = (blockIdx.x + static_cast<long long>(b) * hkv + h) * p.groups;
-    const bool failed = *cta_abort != 0;
+    if (!ok) break;
+  }
+  // after a wait that gave up: the copies in flight land before the shared memory is given back (or this wait gives up too),
+  // and what this warp would still have finished is NaN
+  if (!ok) {
+    for (int x = xc; x < xi; ++x) {
+      const uint64_t t0 = globaltimer_ns();
+      while (!mbar_try_wait(bars + 8 * st, parity) && globaltimer_ns() - t0 < kWaitLimitNs) {}
+      if (++st == S) { st = 0; parity ^= 1; }
+    }
+    for (int x = xw0; x < xw1;) {
+      const int bb = seq_of(x), n = pre[bb + 1] - pre[bb], h = (x - pre[bb] * hkv) / n, first = pre[bb] * hkv + h * n;
+      for (int i = lane; i < p.groups * D; i += 32) {
+        store_o(bb, h * p.groups + i / D, i % D, __int_as_float(0x7fc00000));
+        if (p.lse && i % D == 0) p.lse[static_cast<long long>(bb) * p.hq + h * p.groups + i / D] = __int_as_float(0x7fc00000);
+      }
+      x = first + n;
+    }
+  }
+
+  // ---- pieces of one segment are joined, warps in order
+  __syncthreads();
+  const bool failed = *cta_abort != 0;
+  for (int e0 = 0; e0 < 2 * W;) {
+    const int seg = seg_of[e0];
+    if (seg < 0) { ++e0; continue; }
+    int e1 = e0 + 1;
+    while (e1 < 2 * W && (seg_of[e1] < 0 || seg_of[e1] == seg)) ++e1;
+    const int sb = seg / hkv, h = seg % hkv, n = pre[sb + 1] - pre[sb], first = pre[sb] * hkv + h * n;
+    const bool inside = first >= x0 && first + n <= x1;
+    const long long part = (static_cast<long long>(blockIdx.x) + seg) * p.groups;
     for (int i = tid; i < p.groups * D; i += NTHR) {
       const int head = i / D, d = i % D;
       float top = -INFINITY, den = 0.0f, acc = 0.0f;
-#pragma unroll
-      for (int w = 0; w < W; ++w) top = fmaxf(top, ml[w * H + head]);
-#pragma unroll
-      for (int w = 0; w < W; ++w) {
-        const float lw = ml[(W + w) * H + head], mw = ml[w * H + head];
-        if (lw != 0.0f) {  // a warp without keys here has written nothing else
-          const float f = ex2_approx(mw == -INFINITY ? 0.0f : mw - top);
-          den += f * lw;
-          acc += f * red[(w * H + head) * D + d];
-        }
+      for (int e = e0; e < e1; ++e)
+        if (seg_of[e] >= 0) top = fmaxf(top, ml[e * H + head]);
+      for (int e = e0; e < e1; ++e) {
+        if (seg_of[e] < 0) continue;
+        const float mw = ml[e * H + head], lw = ml[(2 * W + e) * H + head];
+        if (lw == 0.0f) continue;
+        const float* from = (e & 1) ? reinterpret_cast<const float*>(smem + (e >> 1) * C::kRingWarp)
+                                    : p.piece_o + (static_cast<long long>(blockIdx.x) * W + (e >> 1)) * p.groups * D;
+        const float f = ex2_approx(mw == -INFINITY ? 0.0f : mw - top);
+        den += f * lw;
+        acc += f * from[i];
       }
-      const float nan = __int_as_float(0x7fc00000);
       float val = den != 0.0f ? acc / den : 0.0f;
-      // 2^14 of the weights; a NaN sum has no maximum of its own
       float lse = den != 0.0f ? log2f(den) - 14.0f + (top == -INFINITY ? 0.0f : top) : -INFINITY;
-      if (failed) val = lse = nan;
-      if (whole) {
-        store_o(b, h * p.groups + head, d, val);
-        if (d == 0 && p.lse) p.lse[static_cast<long long>(b) * p.hq + h * p.groups + head] = lse;
+      if (failed) val = lse = __int_as_float(0x7fc00000);
+      if (inside) {
+        store_o(sb, h * p.groups + head, d, val);
+        if (d == 0 && p.lse) p.lse[static_cast<long long>(sb) * p.hq + h * p.groups + head] = lse;
       } else {
         p.part_o[(part + head) * D + d] = val;
         if (d == 0) p.part_lse[part + head] = lse;
       }
     }
-    seg_x = seg_end;
+    e0 = e1;
   }
-  // after a wait that gave up: the copies in flight land before the shared memory is given back (or this wait gives up too)
-  if (!ok)
-    for (; xc < xi; xc += W) {
-      const uint64_t t0 = globaltimer_ns();
-      while (!mbar_try_wait(bars + 8 * st, parity) && globaltimer_ns() - t0 < kWaitLimitNs) {}
-      if (++st == S) { st = 0; parity ^= 1; }
-    }
 }
 
-// Joins the partial results of segments that were cut: one CTA per query head.  Segment s = b * Hkv + h of tiles
-// [first, last) has a part from each of the CTAs first / per .. (last - 1) / per, at index CTA + s.
+// Joins the partial results of segments that lie in several CTAs.  Segment s = b * Hkv + h of tiles [first, last) has a part
+// from each of the CTAs first / per .. (last - 1) / per, at index CTA + s.  A CTA here takes one query head: of every segment
+// (grid Hq x B), or where there are more segments than cuts of the segment that is cut first at CTA y + 1 (grid group x cuts).
 template <int D>
-__global__ void __launch_bounds__(128 * kMergeGroups) paged_merge_kernel(const __grid_constant__ PagedDecodeParams p) {
+__global__ void __launch_bounds__(128 * kMergeGroups) paged_merge_kernel(const __grid_constant__ PagedDecodeParams p, const int by_cut) {
   __shared__ MergeScratch sm;
   griddep_launch();
   griddep_wait();
-  const int hq = blockIdx.x, b = blockIdx.y, h = hq / p.groups;
   const bool failed = cta_device_failed();
+  int b = blockIdx.y, h = blockIdx.x / p.groups;
+  const int head = blockIdx.x % p.groups;
+  if (by_cut) {
+    const int seg = p.cut[blockIdx.y + 1];
+    if (failed) {   // then there may be no cuts: some CTA or other writes every row
+      for (long long row = blockIdx.y; row < static_cast<long long>(p.batch) * p.pool.hkv; row += gridDim.y)
+        if (threadIdx.x < D) {
+          const int rb = static_cast<int>(row / p.pool.hkv), hq = static_cast<int>(row % p.pool.hkv) * p.groups + head;
+          const float nan = __int_as_float(0x7fc00000);
+          reinterpret_cast<uint16_t*>(p.o)[rb * p.o_sb + hq * p.o_sh + threadIdx.x] = p.o_bf16 ? from_f32<true>(nan) : from_f32<false>(nan);
+          if (threadIdx.x == 0 && p.lse) p.lse[static_cast<long long>(rb) * p.hq + hq] = nan;
+        }
+      return;
+    }
+    if (seg < 0) return;
+    b = seg / p.pool.hkv;
+    h = seg % p.pool.hkv;
+  }
+  const int hq = h * p.groups + head;
   float val = __int_as_float(0x7fc00000), lse = val;
   if (!failed) {
     const int n = p.plan[b + 1] - p.plan[b], per = p.plan[p.batch + 1];
     if (n == 0) return;
-    const long long first = static_cast<long long>(p.plan[b]) * p.pool.hkv + static_cast<long long>(h) * n;
-    const long long c0 = first / per, c1 = (first + n - 1) / per;
+    const int first = p.plan[b] * p.pool.hkv + h * n;
+    const int c0 = first / per, c1 = (first + n - 1) / per;
     if (c0 == c1) return;
-    const long long base = (c0 + static_cast<long long>(b) * p.pool.hkv + h) * p.groups + hq % p.groups;
-    merge_row_partials(p.part_o, p.part_lse, base, p.groups, static_cast<int>(c1 - c0 + 1), D, sm, val, lse);
+    const long long base = (static_cast<long long>(c0) + b * p.pool.hkv + h) * p.groups + head;
+    merge_row_partials(p.part_o, p.part_lse, base, p.groups, c1 - c0 + 1, D, sm, val, lse);
   }
   if (threadIdx.x < D) {
     reinterpret_cast<uint16_t*>(p.o)[b * p.o_sb + hq * p.o_sh + threadIdx.x] = p.o_bf16 ? from_f32<true>(val) : from_f32<false>(val);

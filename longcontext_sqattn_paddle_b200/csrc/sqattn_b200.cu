@@ -618,30 +618,41 @@ int paged_decode_check(const sqattn_paged_decode_args* a) {
   return SQATTN_OK;
 }
 
-// scratch of a paged decode: [part_o | part_lse | plan]
+// scratch of a paged decode: [part_o | part_lse | piece_o | plan | cut]
 struct PagedDecodePlan {
-  int grid, min_tiles, max_len;
-  size_t parts, lse_off, plan_off, total;
+  int grid, max_len;
+  size_t lse_off, piece_off, plan_off, cut_off, total;
 };
+template <int FMT, int D, int NT>
+void paged_decode_shape(int* tile, int* warps) {
+  *tile = PagedDecodeCfg<FMT, D, NT>::kTile;
+  *warps = PagedDecodeCfg<FMT, D, NT>::kWarps;
+}
 int plan_paged_decode(const sqattn_paged_decode_args* a, PagedDecodePlan* pl) {
   int rc;
   if ((rc = paged_decode_check(a))) return rc;
   const sqattn_paged_pool* pool = a->pool;
   if (a->batch > kPagedMaxBatch) return fail(SQATTN_ERR_UNSUPPORTED, "paged decode: at most %d sequences a call, got %d", kPagedMaxBatch, a->batch);
+  const int groups = a->num_q_heads / pool->num_kv_heads;
+  int tile = 0, warps = 0;
+#define SQ_LAUNCH(F, D, B) (groups > 8 ? paged_decode_shape<F, D, 2> : paged_decode_shape<F, D, 1>)(&tile, &warps)
+  SQ_PAGED_DISPATCH(pool, SQ_LAUNCH);
+#undef SQ_LAUNCH
   const int64_t cap = std::min<int64_t>(static_cast<int64_t>(a->max_pages) * pool->page_size, 0x7fffff00ll);
   pl->max_len = static_cast<int>(a->max_kv_len ? std::min<int64_t>(cap, a->max_kv_len) : cap);
   const int64_t keys = a->pages ? static_cast<int64_t>(a->num_listed) * pool->page_size : pl->max_len;
-  const int64_t tiles = (keys + kPagedTile - 1) / kPagedTile * pool->num_kv_heads;
-  if (keys > 0x7fffff00ll || tiles > 2147483647ll / a->batch)
+  const int64_t tiles = (keys + tile - 1) / tile * pool->num_kv_heads;
+  if (keys > 0x7fffff00ll || tiles > 0x7fff0000ll / a->batch)
     return fail(SQATTN_ERR_UNSUPPORTED, "paged decode: %d sequences of up to %lld keys and %d KV heads are more than a call takes (max_kv_len bounds the keys)",
                 a->batch, static_cast<long long>(keys), pool->num_kv_heads);
-  pl->min_tiles = (pool->format == SQATTN_KV_NATIVE && pool->head_dim == 128) ? 4 : 8;   // one for each warp
-  pl->grid = static_cast<int>(std::min<int64_t>(148, (tiles * a->batch + pl->min_tiles - 1) / pl->min_tiles));   // one CTA per SM
-  const int groups = a->num_q_heads / pool->num_kv_heads;
-  pl->parts = static_cast<size_t>(pl->grid) + static_cast<size_t>(a->batch) * pool->num_kv_heads;
-  pl->lse_off = align_up(pl->parts * groups * pool->head_dim * 4, 256);
-  pl->plan_off = pl->lse_off + align_up(pl->parts * groups * 4, 256);
-  pl->total = pl->plan_off + align_up((static_cast<size_t>(a->batch) + 2) * 4, 256);
+  pl->grid = static_cast<int>(std::min<int64_t>(148, (tiles * a->batch + warps - 1) / warps));   // one CTA per SM, a tile for every warp
+  const size_t row = static_cast<size_t>(groups) * pool->head_dim * 4;
+  const size_t parts = static_cast<size_t>(pl->grid) + static_cast<size_t>(a->batch) * pool->num_kv_heads;
+  pl->lse_off = align_up(parts * row, 256);
+  pl->piece_off = pl->lse_off + align_up(parts * groups * 4, 256);
+  pl->plan_off = pl->piece_off + align_up(static_cast<size_t>(pl->grid) * warps * row, 256);
+  pl->cut_off = pl->plan_off + align_up((static_cast<size_t>(a->batch) + 2) * 4, 256);
+  pl->total = pl->cut_off + align_up(static_cast<size_t>(pl->grid) * 4, 256);
   return SQATTN_OK;
 }
 
@@ -666,7 +677,7 @@ int make_tmap_pages(CUtensorMap* out, const void* ptr, const sqattn_paged_pool* 
 template <int FMT, int D, bool BF16, int NT>
 int launch_paged_decode(const sqattn_paged_decode_args* a, const PagedDecodePlan& pl, const PagedDecodeParams& p, cudaStream_t stream) {
   using Cfg = PagedDecodeCfg<FMT, D, NT>;
-  const int box_rows = (FMT == kKvNative || a->pool->page_size == 16) ? 16 : 32;
+  const int box_rows = FMT == kKvNative ? 16 : std::min(a->pool->page_size, Cfg::kTile);
   CUtensorMap tk, tv;
   int rc;
   if ((rc = make_tmap_pages(&tk, a->pool->k_pages, a->pool, Cfg::kRow, box_rows, "k_pages"))) return rc;
@@ -674,8 +685,11 @@ int launch_paged_decode(const sqattn_paged_decode_args* a, const PagedDecodePlan
   SQ_CUDA(cudaFuncSetAttribute(paged_decode_kernel<FMT, D, BF16, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::total(a->batch)));
   paged_decode_kernel<FMT, D, BF16, NT><<<pl.grid, Cfg::kWarps * 32, Cfg::total(a->batch), stream>>>(tk, tv, p);
   SQ_CUDA(cudaGetLastError());
-  if (pl.grid > 1)
-    SQ_CUDA(launch_overlapped(1, paged_merge_kernel<D>, dim3(a->num_q_heads, a->batch), dim3(128 * kMergeGroups), 0, stream, p));
+  if (pl.grid > 1) {
+    const int by_cut = (pl.grid - 1) * p.groups < a->num_q_heads * a->batch;
+    const dim3 grid = by_cut ? dim3(p.groups, pl.grid - 1) : dim3(a->num_q_heads, a->batch);
+    SQ_CUDA(launch_overlapped(1, paged_merge_kernel<D>, grid, dim3(128 * kMergeGroups), 0, stream, p, by_cut));
+  }
   return SQATTN_OK;
 }
 
@@ -1416,7 +1430,8 @@ int sqattn_paged_decode(const sqattn_paged_decode_args* a, sqattn_stream_t strea
   if ((rc = plan_paged_decode(a, &pl))) return rc;
   const sqattn_paged_pool* pool = a->pool;
   if (!a->q.ptr || !a->o.ptr) return fail(SQATTN_ERR_INVALID_ARG, "paged decode: null tensor pointer");
-  if ((reinterpret_cast<uintptr_t>(a->q.ptr) | reinterpret_cast<uintptr_t>(a->o.ptr)) & 1) return fail(SQATTN_ERR_INVALID_ARG, "paged decode: q and o need 2-byte alignment");
+  if (reinterpret_cast<uintptr_t>(a->q.ptr) % 2) return fail(SQATTN_ERR_INVALID_ARG, "paged decode: q needs 2-byte alignment");
+  if (reinterpret_cast<uintptr_t>(a->o.ptr) % 4 || a->o.stride_b % 2 || a->o.stride_h % 2) return fail(SQATTN_ERR_INVALID_ARG, "paged decode: o needs 4-byte alignment");
   if (!a->workspace || a->workspace_bytes < pl.total || (reinterpret_cast<uintptr_t>(a->workspace) % 256))
     return fail(SQATTN_ERR_WORKSPACE, "workspace of %zu bytes (256-byte aligned) required", pl.total);
   PagedDecodeParams p;
@@ -1426,7 +1441,7 @@ int sqattn_paged_decode(const sqattn_paged_decode_args* a, sqattn_stream_t strea
   p.q = static_cast<const uint8_t*>(a->q.ptr); p.q_sb = a->q.stride_b; p.q_sh = a->q.stride_h;
   p.o = static_cast<uint8_t*>(a->o.ptr); p.o_sb = a->o.stride_b; p.o_sh = a->o.stride_h;
   p.lse = a->lse; p.kv_lens = a->kv_lens; p.list = a->pages; p.list_len = a->num_listed;
-  p.max_len = pl.max_len; p.min_tiles = pl.min_tiles;
+  p.max_len = pl.max_len;
   p.batch = a->batch; p.hq = a->num_q_heads; p.groups = a->num_q_heads / pool->num_kv_heads;
   p.q_bf16 = pool->dtype == SQATTN_BF16; p.o_bf16 = a->o_dtype == SQATTN_BF16;
   const double scale = a->sm_scale > 0.0f ? static_cast<double>(a->sm_scale) : 1.0 / sqrt(static_cast<double>(pool->head_dim));
@@ -1434,7 +1449,9 @@ int sqattn_paged_decode(const sqattn_paged_decode_args* a, sqattn_stream_t strea
   uint8_t* ws = static_cast<uint8_t*>(a->workspace);
   p.part_o = reinterpret_cast<float*>(ws);
   p.part_lse = reinterpret_cast<float*>(ws + pl.lse_off);
+  p.piece_o = reinterpret_cast<float*>(ws + pl.piece_off);
   p.plan = reinterpret_cast<int*>(ws + pl.plan_off);
+  p.cut = reinterpret_cast<int*>(ws + pl.cut_off);
   // codes become f16 whatever the queries' type
 #define SQ_LAUNCH(F, D, B) \
   return p.groups > 8 ? launch_paged_decode<F, D, (F) == kKvNative && B, 2>(a, pl, p, stream) : launch_paged_decode<F, D, (F) == kKvNative && B, 1>(a, pl, p, stream)

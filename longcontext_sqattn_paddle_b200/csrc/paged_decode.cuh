@@ -68,7 +68,7 @@ struct PagedDecodeCfg {
   static constexpr int kBarOff = kMlOff + 2 * kWarps * 8 * NT * 8;       // [warp][stage]
   static constexpr int kInfoOff = kBarOff + kWarps * kStages * 8;        // [warp][stage] valid keys
   static constexpr int kSegOff = kInfoOff + kWarps * kStages * 4;        // [2 warps] segments of the pieces
-  static constexpr int kMiscOff = kSegOff + 2 * kWarps * 4;              // abort flag
+  static constexpr int kMiscOff = kSegOff + 2 * kWarps * 4;              // abort flag, exponents of codes
   static constexpr int kPlanOff = (kMiscOff + 16 + 15) / 16 * 16;        // [B + 1]
   static constexpr int total(int batch) { return kPlanOff + (batch + 1) * 4 + 1024; }
   static_assert(total(kPagedMaxBatch) <= 227 * 1024, "shared memory of a CTA");
@@ -97,15 +97,18 @@ __device__ __forceinline__ uint32_t h2_fma(uint32_t a, uint32_t b, uint32_t c) {
 }
 // Codes to f16 pairs, exactly.  The bits of a biased code (sign bit flipped) under the exponent of 1024 are 1024 + code + bias.
 //   bytes 0, 2 of x / bytes 1, 3 of x;   nibbles 0, 4 / 1, 5 / 2, 6 / 3, 7 of x (the odd ones arrive 16 times as large)
-__device__ __forceinline__ void bytes_to_h2(uint32_t x, uint32_t& even, uint32_t& odd) {
+// One of the two constants of (x & mask) ^ exponent has to be in a register for one instruction to do it: the exponents come
+// from memory, so that the compiler cannot make them immediates (which then take two instructions).
+struct CodeExponents { uint32_t low, high; };  // 0x64086408, 0x64806480
+__device__ __forceinline__ void bytes_to_h2(uint32_t x, const CodeExponents& ce, uint32_t& even, uint32_t& odd) {
   constexpr uint32_t kMinus1152 = 0xe480e480u;
-  even = h2_add((x & 0x00ff00ffu) ^ 0x64806480u, kMinus1152);
-  odd = h2_add(((x >> 8) & 0x00ff00ffu) ^ 0x64806480u, kMinus1152);
+  even = h2_add((x & 0x00ff00ffu) ^ ce.high, kMinus1152);
+  odd = h2_add(((x >> 8) & 0x00ff00ffu) ^ ce.high, kMinus1152);
 }
-__device__ __forceinline__ void nibbles_to_h2(uint32_t x, uint32_t& n0, uint32_t& n1) {
+__device__ __forceinline__ void nibbles_to_h2(uint32_t x, const CodeExponents& ce, uint32_t& n0, uint32_t& n1) {
   constexpr uint32_t kMinus1032 = 0xe408e408u, kSixteenth = 0x2c002c00u, kMinus72 = 0xd480d480u;
-  n0 = h2_add((x & 0x000f000fu) ^ 0x64086408u, kMinus1032);
-  n1 = h2_fma((x & 0x00f000f0u) ^ 0x64806480u, kSixteenth, kMinus72);
+  n0 = h2_add((x & 0x000f000fu) ^ ce.low, kMinus1032);
+  n1 = h2_fma((x & 0x00f000f0u) ^ ce.high, kSixteenth, kMinus72);
 }
 
 // Key that row r (0..7; +8 likewise) of a product's 16 keys stands for.  A quarter or half warp reads the rows of four lanes t
@@ -182,7 +185,9 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
   } else if (warp == 1) {
     if (lane < 2 * W) seg_of[lane] = -1;
     if (lane == 0) {
-      *cta_abort = 0;
+      cta_abort[0] = 0;
+      cta_abort[1] = 0x64086408;
+      cta_abort[2] = 0x64806480;
       for (int i = 0; i < W * S; ++i) mbar_init(sbase + C::kBarOff + 8 * i, 1);
       fence_barrier_init();
       fence_proxy_async();
@@ -348,6 +353,10 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
   };
   const int key_row = kNative ? g : row_perm<ROW>(g);  // this lane's first key of 16: that row and the one 8 further
 
+  CodeExponents ce;
+  asm volatile("ld.volatile.shared.u32 %0, [%1];" : "=r"(ce.low) : "r"(sbase + C::kMiscOff + 4));
+  asm volatile("ld.volatile.shared.u32 %0, [%1];" : "=r"(ce.high) : "r"(sbase + C::kMiscOff + 8));
+
   int st = 0;
   uint32_t parity = 0;
   bool ok = true;
@@ -475,16 +484,16 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
             for (int i = 0; i < kWords; ++i) {
               if (FMT == kKvInt8) {
                 uint32_t a[4];
-                bytes_to_h2(w[0][i], a[0], a[2]);
-                bytes_to_h2(w[1][i], a[1], a[3]);
+                bytes_to_h2(w[0][i], ce, a[0], a[2]);
+                bytes_to_h2(w[1][i], ce, a[1], a[3]);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) mma_16816<false>(s[nt][mt], a, qb[nt][i][0], qb[nt][i][1]);
               } else {
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
                   uint32_t a[4];
-                  nibbles_to_h2(w[0][i] >> (8 * u), a[0], a[2]);
-                  nibbles_to_h2(w[1][i] >> (8 * u), a[1], a[3]);
+                  nibbles_to_h2(w[0][i] >> (8 * u), ce, a[0], a[2]);
+                  nibbles_to_h2(w[1][i] >> (8 * u), ce, a[1], a[3]);
 #pragma unroll
                   for (int nt = 0; nt < NT; ++nt) mma_16816<false>(s[nt][mt], a, qb[nt][2 * i + u][0], qb[nt][2 * i + u][1]);
                 }
@@ -629,16 +638,16 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
                 const uint32_t hi = __byte_perm(w[2][u], w[3][u], half ? 0x7632 : 0x5410);
                 if (FMT == kKvInt8) {
                   uint32_t a[4];
-                  bytes_to_h2(lo, a[0], a[1]);
-                  bytes_to_h2(hi, a[2], a[3]);
+                  bytes_to_h2(lo, ce, a[0], a[1]);
+                  bytes_to_h2(hi, ce, a[2], a[3]);
 #pragma unroll
                   for (int nt = 0; nt < NT; ++nt) mma_16816<false>(o[nt][2 * u + half], a, pb[nt][mt][0], pb[nt][mt][1]);
                 } else {
 #pragma unroll
                   for (int q = 0; q < 2; ++q) {
                     uint32_t a[4];
-                    nibbles_to_h2(lo >> (8 * q), a[0], a[1]);
-                    nibbles_to_h2(hi >> (8 * q), a[2], a[3]);
+                    nibbles_to_h2(lo >> (8 * q), ce, a[0], a[1]);
+                    nibbles_to_h2(hi >> (8 * q), ce, a[2], a[3]);
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) mma_16816<false>(o[nt][4 * u + 2 * half + q], a, pb[nt][mt][0], pb[nt][mt][1]);
                   }

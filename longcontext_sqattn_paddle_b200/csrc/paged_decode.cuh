@@ -17,9 +17,13 @@
 // the 8 columns: with at most 8 heads to a group no product is padding but the unused heads' columns.  The products do not
 // bound the kernel (a key takes 0.25 KFLOP a head for 128-512 bytes), so the tcgen05 path, which would need 64 or 128
 // rows of queries, has nothing to give here.
-//   codes: int8 and 4-bit codes become f16 exactly by exponent tricks; q is brought to f16 by a power of two per head
-//     (bf16's 8 bits are kept), a key's scale multiplies its scores and a value's scale its weight p, in fp32.  The weight
-//     p * scale is rounded to f16 relative to the largest value scale so far (as a power of two), 2^14 high.
+//   codes, scores: integer products m16n8k32 of the keys' bytes as they lie (4-bit codes as the high halves of bytes: a mask) with
+//     q as 16-bit integers, a power of two per head high, in a signed high and an unsigned low byte: sums are exact, and q is
+//     off by at most 2^-15 of the head's largest (bf16 channels down to 1/64 of the largest are exact).
+//   codes, output: codes become f16 exactly by exponent tricks; a value's scale multiplies its weight p in fp32, and the product
+//     is rounded to f16 relative to the largest value scale so far (as a power of two), 2^14 high.
+//   The conversions are what costs: on this part an ALU or f16x2 instruction takes an SM quarter 2 clocks, a f16 product
+//     m16n8k16 8.3, an integer product m16n8k32 8.1, and they hardly overlap.
 //   native: p is split into two 16-bit parts, so that its rounding (2^-16 or 2^-22) vanishes beside the output's.
 // Channels and keys may enter a product in any order as long as both operands agree, so codes are taken from shared memory
 // in the order in which they lie (16 bytes a lane); `row_perm` below orders the keys so that those loads do not collide.
@@ -59,7 +63,7 @@ struct PagedDecodeCfg {
   static constexpr int kRow = kv_row_bytes<FMT>(D);
   static constexpr int kTile = FMT == kKvInt4 ? 64 : 32;                 // keys of a tile
   static constexpr int kWarps = FMT == kKvNative ? (D == 128 ? 4 : 8) : (NT == 2 ? 8 : 12);
-  static constexpr int kStages = FMT == kKvNative ? 3 : 2;
+  static constexpr int kStages = 2;
   static constexpr int kTensor = kTile * kRow;                           // a tile's keys or values
   static constexpr int kRingWarp = kStages * 2 * kTensor;
   static constexpr int kScaleOff = kWarps * kRingWarp;                   // [warp][stage][K, V][kTile] fp32
@@ -67,7 +71,8 @@ struct PagedDecodeCfg {
   static constexpr int kMlOff = kScaleOff + kWarps * kStages * kScaleStage;  // [2 warps][8 NT] maxima, then sums
   static constexpr int kBarOff = kMlOff + 2 * kWarps * 8 * NT * 8;       // [warp][stage]
   static constexpr int kInfoOff = kBarOff + kWarps * kStages * 8;        // [warp][stage] valid keys
-  static constexpr int kSegOff = kInfoOff + kWarps * kStages * 4;        // [2 warps] segments of the pieces
+  static constexpr int kRecOff = (kInfoOff + kWarps * kStages * 4 + 15) / 16 * 16;  // [warp][32 tiles] where their pages lie
+  static constexpr int kSegOff = kRecOff + kWarps * 32 * 32;             // [2 warps] segments of the pieces
   static constexpr int kMiscOff = kSegOff + 2 * kWarps * 4;              // abort flag, exponents of codes
   static constexpr int kPlanOff = (kMiscOff + 16 + 15) / 16 * 16;        // [B + 1]
   static constexpr int total(int batch) { return kPlanOff + (batch + 1) * 4 + 1024; }
@@ -75,10 +80,15 @@ struct PagedDecodeCfg {
   static_assert(8 * NT * D * 4 <= kRingWarp, "a warp's last piece takes the place of its ring");
 };
 
-// untiled copy global -> shared, completion counted in bytes on `bar`
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
-               : "memory");
+// C[16][8] += A[16][32] B[32][8] in integers: signed bytes by the signed high bytes (kHigh) or the unsigned low bytes of 16-bit numbers
+template <bool kHigh>
+__device__ __forceinline__ void mma_16832_int(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  if (kHigh)
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.u8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t a) {
   uint32_t r;
@@ -90,25 +100,22 @@ __device__ __forceinline__ uint32_t h2_add(uint32_t a, uint32_t b) {
   asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
-__device__ __forceinline__ uint32_t h2_fma(uint32_t a, uint32_t b, uint32_t c) {
-  uint32_t r;
-  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
-  return r;
-}
-// Codes to f16 pairs, exactly.  The bits of a biased code (sign bit flipped) under the exponent of 1024 are 1024 + code + bias.
-//   bytes 0, 2 of x / bytes 1, 3 of x;   nibbles 0, 4 / 1, 5 / 2, 6 / 3, 7 of x (the odd ones arrive 16 times as large)
+// Codes to f16 pairs, exactly.  The bits of a biased code (sign bit flipped) under the exponent of 1024 are 1024 + code + bias;
+// four bits further up they are 64 + code + bias under the exponent of 64.
+//   bytes 0, 2 of x / bytes 1, 3 of x;   nibbles 0, 4 / 1, 5 of x
 // One of the two constants of (x & mask) ^ exponent has to be in a register for one instruction to do it: the exponents come
 // from memory, so that the compiler cannot make them immediates (which then take two instructions).
-struct CodeExponents { uint32_t low, high; };  // 0x64086408, 0x64806480
+struct CodeExponents { uint32_t byte, low, high; };  // of 1024 for bytes and low nibbles, of 64 for nibbles 4 bits up; bias in it
+constexpr uint32_t kByteExponent = 0x64806480u, kLowExponent = 0x64086408u, kHighExponent = 0x54805480u;
 __device__ __forceinline__ void bytes_to_h2(uint32_t x, const CodeExponents& ce, uint32_t& even, uint32_t& odd) {
   constexpr uint32_t kMinus1152 = 0xe480e480u;
-  even = h2_add((x & 0x00ff00ffu) ^ ce.high, kMinus1152);
-  odd = h2_add(((x >> 8) & 0x00ff00ffu) ^ ce.high, kMinus1152);
+  even = h2_add((x & 0x00ff00ffu) ^ ce.byte, kMinus1152);
+  odd = h2_add(((x >> 8) & 0x00ff00ffu) ^ ce.byte, kMinus1152);
 }
 __device__ __forceinline__ void nibbles_to_h2(uint32_t x, const CodeExponents& ce, uint32_t& n0, uint32_t& n1) {
-  constexpr uint32_t kMinus1032 = 0xe408e408u, kSixteenth = 0x2c002c00u, kMinus72 = 0xd480d480u;
+  constexpr uint32_t kMinus1032 = 0xe408e408u, kMinus72 = 0xd480d480u;
   n0 = h2_add((x & 0x000f000fu) ^ ce.low, kMinus1032);
-  n1 = h2_fma((x & 0x00f000f0u) ^ ce.high, kSixteenth, kMinus72);
+  n1 = h2_add((x & 0x00f000f0u) ^ ce.high, kMinus72);
 }
 
 // Key that row r (0..7; +8 likewise) of a product's 16 keys stands for.  A quarter or half warp reads the rows of four lanes t
@@ -186,9 +193,10 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     if (lane < 2 * W) seg_of[lane] = -1;
     if (lane == 0) {
       cta_abort[0] = 0;
-      cta_abort[1] = 0x64086408;
-      cta_abort[2] = 0x64806480;
-      for (int i = 0; i < W * S; ++i) mbar_init(sbase + C::kBarOff + 8 * i, 1);
+      cta_abort[1] = kByteExponent;
+      cta_abort[2] = kLowExponent;
+      cta_abort[3] = kHighExponent;
+      for (int i = 0; i < W * S; ++i) mbar_init(sbase + C::kBarOff + 8 * i, kNative ? 1 : 33);  // codes: every lane's scales, too
       fence_barrier_init();
       fence_proxy_async();
     }
@@ -244,41 +252,41 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
   }
 
   // ---- copies.  Lane i looks up the i-th of the warp's next 32 tiles: for each 16 keys of it page * Hkv + head and the number of
-  // valid ones (8 bits each), and the first row inside the page (pages of fewer rows than a tile begin at their row 0)
+  // valid ones (8 bits each), and the first row inside the page (pages of fewer rows than a tile begin at their row 0).  Scales
+  // come by 16-byte copies of the lanes: as bulk copies, of 64 to 256 bytes each, they took as many instructions again as the rows
   const int ps = 1 << p.pool.ps_shift;
   const uint32_t ring = sbase + warp * C::kRingWarp;
   const uint32_t scales = sbase + C::kScaleOff + warp * S * C::kScaleStage;
   const int box = kNative ? 16 : min(ps, TILE);   // rows of a copy, as the tensor maps have it
-  int rec_ph[MT], rec_row = 0;
-  uint32_t rec_nv = 0;
+  uint32_t* rec = reinterpret_cast<uint32_t*>(smem + C::kRecOff) + warp * 256;   // [tile][4 pages, first row, valid keys]
   auto look_up = [&](int x) {
+    uint32_t* mine = rec + lane * 8;
+    uint32_t nv = 0;
+    if (x < xw1) {
+      const int b = seq_of(x);
+      const int n = pre[b + 1] - pre[b], rem = x - pre[b] * hkv;
+      const int h = rem / n, key = (rem - h * n) * TILE;
+      const int len = paged_len(p, b);
+      const int held = static_cast<int>((static_cast<unsigned>(len) + ps - 1) >> p.pool.ps_shift);
+      int at_last = -1, ph = 0, first = 0;
 #pragma unroll
-    for (int s = 0; s < MT; ++s) rec_ph[s] = 0;
-    rec_row = 0;
-    rec_nv = 0;
-    if (x >= xw1) return;
-    const int b = seq_of(x);
-    const int n = pre[b + 1] - pre[b], rem = x - pre[b] * hkv;
-    const int h = rem / n, key = (rem - h * n) * TILE;
-    const int len = paged_len(p, b);
-    const int held = static_cast<int>((static_cast<unsigned>(len) + ps - 1) >> p.pool.ps_shift);
-    rec_row = key & (ps - 1);
-    int at_last = -1, ph = 0, first = 0;
-#pragma unroll
-    for (int s = 0; s < MT; ++s) {
-      const int at = static_cast<int>(static_cast<unsigned>(key + 16 * s) >> p.pool.ps_shift);
-      if (at != at_last) {
-        at_last = at;
-        int index = at;
-        if (p.list) index = at < p.list_len ? p.list[(static_cast<long long>(b) * hkv + h) * p.list_len + at] : -1;
-        const int page = index >= 0 && index < held ? page_of(p.table, b, index, p.pool.num_pages) : -1;
-        ph = page * hkv + h;
-        first = page >= 0 ? index << p.pool.ps_shift : len;   // position of the page's row 0
+      for (int s = 0; s < MT; ++s) {
+        const int at = static_cast<int>(static_cast<unsigned>(key + 16 * s) >> p.pool.ps_shift);
+        if (at != at_last) {
+          at_last = at;
+          int index = at;
+          if (p.list) index = at < p.list_len ? p.list[(static_cast<long long>(b) * hkv + h) * p.list_len + at] : -1;
+          const int page = index >= 0 && index < held ? page_of(p.table, b, index, p.pool.num_pages) : -1;
+          ph = page * hkv + h;
+          first = page >= 0 ? index << p.pool.ps_shift : len;   // position of the page's row 0
+        }
+        mine[s] = ph;
+        const int left = len - first - ((key + 16 * s) & (ps - 1));
+        nv |= static_cast<uint32_t>(min(max(left, 0), 16)) << (8 * s);
       }
-      rec_ph[s] = ph;
-      const int left = len - first - ((key + 16 * s) & (ps - 1));
-      rec_nv |= static_cast<uint32_t>(min(max(left, 0), 16)) << (8 * s);
+      mine[4] = key & (ps - 1);
     }
+    mine[5] = nv;
   };
   int xi = xw0, ahead = 32;  // next tile to copy, its place among the looked-up ones
   auto issue = [&](int st) {
@@ -286,29 +294,38 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     if (ahead == 32) {
       look_up(xi + lane * step);
       ahead = 0;
+      __syncwarp();
     }
-    if (lane == ahead) {
-      info[st] = rec_nv;
-      const uint32_t bar = bars + 8 * st, dst = ring + st * (2 * C::kTensor), sdst = scales + st * C::kScaleStage;
-      const int step = box >> 4;   // in units of 16 rows
+    const uint32_t* r = rec + ahead * 8;
+    const uint32_t nv = r[5];
+    const int row0 = r[4];
+    const uint32_t bar = bars + 8 * st;
+    if (lane == 0) {
+      info[st] = nv;
+      const uint32_t dst = ring + st * (2 * C::kTensor);
+      const int every = box >> 4;   // in units of 16 rows
       // valid rows come first in a page, so a box has some if its first 16 have
       int boxes = 0;
 #pragma unroll
-      for (int s = 0; s < MT; ++s) boxes += (s & (step - 1)) == 0 && ((rec_nv >> (8 * s)) & 0xffu) != 0u;
-      mbar_expect_tx(bar, boxes * box * (2 * ROW + (kNative ? 0 : 8)));
+      for (int s = 0; s < MT; ++s) boxes += (s & (every - 1)) == 0 && ((nv >> (8 * s)) & 0xffu) != 0u;
+      mbar_expect_tx(bar, boxes * box * (2 * ROW));
 #pragma unroll
       for (int s = 0; s < MT; ++s)
-        if ((s & (step - 1)) == 0 && ((rec_nv >> (8 * s)) & 0xffu) != 0u) {
-          const int row = (rec_row + 16 * s) & (ps - 1);
-          const int line = kNative ? row : row * ROW / 128;
-          tma_load_4d(dst + s * (16 * ROW), &tm_k, bar, 0, line, 0, rec_ph[s]);
-          tma_load_4d(dst + C::kTensor + s * (16 * ROW), &tm_v, bar, 0, line, 0, rec_ph[s]);
-          if (!kNative) {
-            const long long off = (static_cast<long long>(rec_ph[s]) << p.pool.ps_shift) + row;
-            bulk_load(sdst + s * 64, p.pool.k_scale + off, box * 4, bar);
-            bulk_load(sdst + (TILE + s * 16) * 4, p.pool.v_scale + off, box * 4, bar);
-          }
+        if ((s & (every - 1)) == 0 && ((nv >> (8 * s)) & 0xffu) != 0u) {
+          const int row = (row0 + 16 * s) & (ps - 1), line = kNative ? row : row * ROW / 128;
+          tma_load_4d(dst + s * (16 * ROW), &tm_k, bar, 0, line, 0, r[s]);
+          tma_load_4d(dst + C::kTensor + s * (16 * ROW), &tm_v, bar, 0, line, 0, r[s]);
         }
+    }
+    if (!kNative) {
+      // scales of four keys a lane: the keys' by the first TILE / 4 lanes, the values' by the next
+      const int c = lane & (TILE / 4 - 1), s = c >> 2, which = lane / (TILE / 4);
+      if (which < 2 && ((nv >> (8 * s)) & 0xffu) != 0u) {
+        const float* src = which ? p.pool.v_scale : p.pool.k_scale;
+        src += (static_cast<long long>(r[s]) << p.pool.ps_shift) + ((row0 + 16 * s) & (ps - 1)) + 4 * (c & 3);
+        cp_async_16(scales + st * C::kScaleStage + which * (TILE * 4) + c * 16, src);
+      }
+      cp_async_arrive(bar);
     }
     ++ahead;
     xi += step;
@@ -354,8 +371,9 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
   const int key_row = kNative ? g : row_perm<ROW>(g);  // this lane's first key of 16: that row and the one 8 further
 
   CodeExponents ce;
-  asm volatile("ld.volatile.shared.u32 %0, [%1];" : "=r"(ce.low) : "r"(sbase + C::kMiscOff + 4));
-  asm volatile("ld.volatile.shared.u32 %0, [%1];" : "=r"(ce.high) : "r"(sbase + C::kMiscOff + 8));
+  ce.byte = cta_abort[1];
+  ce.low = cta_abort[2];
+  ce.high = cta_abort[3];
 
   int st = 0;
   uint32_t parity = 0;
@@ -371,8 +389,8 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     const bool whole = step == 1 && seg_first >= xw0 && seg_last <= xw1;
 
     // ---- query heads as the products' 8 columns
-    uint32_t qb[NT][D / 16][2];
-    float cs[NT][2];  // score factor of this lane's two columns
+    uint32_t qb[NT][D / 16][2];  // native: [channels 16 i ..][r]; codes: [32 of the channels i / 2, high or low bytes i % 2][r]
+    float cs[NT][2];             // score factor of this lane's two columns
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int head = nt * 8 + g;
@@ -399,21 +417,24 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         }
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        // a power of two brings the largest to [2^13, 2^14)
+        // a power of two brings the largest to [2^14, 2^15); 4-bit codes arrive 16 times as large
         const uint32_t e = max(__float_as_uint(top) >> 23, 27u);
-        const float up = __uint_as_float((267u - e) << 23);
-        const float down = p.scale_log2 * __uint_as_float((e - 13u) << 23);
+        const float up = __uint_as_float((268u - e) << 23);
+        const float down = e == 255u ? __int_as_float(0x7fc00000) : p.scale_log2 * __uint_as_float((e - (FMT == kKvInt4 ? 18u : 14u)) << 23);
 #pragma unroll
-        for (int w = 0; w < D / 16; ++w) {
-          if (FMT == kKvInt8) {   // bytes 0, 2 and 1, 3 of word w
-            qb[nt][w][0] = pack_f16x2(f[4 * w] * up, f[4 * w + 2] * up);
-            qb[nt][w][1] = pack_f16x2(f[4 * w + 1] * up, f[4 * w + 3] * up);
-          } else {                // nibbles 0, 4 and 1, 5, then 2, 6 and 3, 7 of word w / 2
-            const int o = 8 * (w / 2) + 2 * (w & 1);
-            qb[nt][w][0] = pack_f16x2(f[o] * up, f[o + 4] * up);
-            qb[nt][w][1] = pack_f16x2(f[o + 1] * up, f[o + 5] * up);
+        for (int j = 0; j < D / 32; ++j)
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            uint32_t hi = 0, lo = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {   // bytes of word 2 j + r, or even and odd nibbles of word j
+              const uint32_t v = static_cast<uint32_t>(__float2int_rn(f[FMT == kKvInt8 ? 8 * j + 4 * r + i : 8 * j + 2 * i + r] * up));
+              hi |= ((v >> 8) & 0xffu) << (8 * i);
+              lo |= (v & 0xffu) << (8 * i);
+            }
+            qb[nt][2 * j][r] = hi;
+            qb[nt][2 * j + 1][r] = lo;
           }
-        }
         cs[nt][0] = __shfl_sync(0xffffffffu, down, 8 * t);
         cs[nt][1] = __shfl_sync(0xffffffffu, down, 8 * t + 4);
       }
@@ -447,12 +468,12 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         }
         // ---- scores
         float s[NT][MT][4];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int mt = 0; mt < MT; ++mt) s[nt][mt][0] = s[nt][mt][1] = s[nt][mt][2] = s[nt][mt][3] = 0.0f;
         float vs[MT][2];  // value scales of this lane's keys
         if (kNative) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) s[nt][mt][0] = s[nt][mt][1] = s[nt][mt][2] = s[nt][mt][3] = 0.0f;
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk)
 #pragma unroll
@@ -481,23 +502,26 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
                 }
               }
 #pragma unroll
-            for (int i = 0; i < kWords; ++i) {
-              if (FMT == kKvInt8) {
+            for (int nt = 0; nt < NT; ++nt) {
+              int high[4] = {0, 0, 0, 0}, low[4] = {0, 0, 0, 0};
+#pragma unroll
+              for (int j = 0; j < D / 32; ++j) {
                 uint32_t a[4];
-                bytes_to_h2(w[0][i], ce, a[0], a[2]);
-                bytes_to_h2(w[1][i], ce, a[1], a[3]);
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) mma_16816<false>(s[nt][mt], a, qb[nt][i][0], qb[nt][i][1]);
-              } else {
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                  uint32_t a[4];
-                  nibbles_to_h2(w[0][i] >> (8 * u), ce, a[0], a[2]);
-                  nibbles_to_h2(w[1][i] >> (8 * u), ce, a[1], a[3]);
-#pragma unroll
-                  for (int nt = 0; nt < NT; ++nt) mma_16816<false>(s[nt][mt], a, qb[nt][2 * i + u][0], qb[nt][2 * i + u][1]);
+                for (int hi = 0; hi < 2; ++hi) {
+                  if (FMT == kKvInt8) {
+                    a[hi] = w[hi][2 * j];
+                    a[2 + hi] = w[hi][2 * j + 1];
+                  } else {   // nibbles as the high halves of signed bytes: 16 times the code
+                    a[hi] = (w[hi][j] << 4) & 0xf0f0f0f0u;
+                    a[2 + hi] = w[hi][j] & 0xf0f0f0f0u;
+                  }
                 }
+                mma_16832_int<true>(high, a[0], a[1], a[2], a[3], qb[nt][2 * j][0], qb[nt][2 * j][1]);
+                mma_16832_int<false>(low, a[0], a[1], a[2], a[3], qb[nt][2 * j + 1][0], qb[nt][2 * j + 1][1]);
               }
+#pragma unroll
+              for (int e = 0; e < 4; ++e) s[nt][mt][e] = static_cast<float>(high[e] * 256 + low[e]);
             }
           }
           // scales
@@ -732,6 +756,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
   // after a wait that gave up: the copies in flight land before the shared memory is given back (or this wait gives up too),
   // and what this warp would still have finished is NaN
   if (!ok) {
+    asm volatile("cp.async.wait_all;" ::: "memory");
     for (int x = xc; x < xi; x += step) {
       const uint64_t t0 = globaltimer_ns();
       while (!mbar_try_wait(bars + 8 * st, parity) && globaltimer_ns() - t0 < kWaitLimitNs) {}

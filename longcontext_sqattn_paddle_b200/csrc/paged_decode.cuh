@@ -50,6 +50,7 @@ struct PagedDecodeParams {
   int list_len;
   int max_len;  // what the table, or the caller's bound, holds
   int batch, hq, groups, q_bf16, o_bf16;
+  int q_align;       // bytes that every head's row is aligned to: 16, 4 or 2
   float scale_log2;  // softmax scale * log2(e)
   float* part_o;     // [grid + B * Hkv, groups, D] fp32, each divided by its own sum
   float* part_lse;   // [grid + B * Hkv, groups]
@@ -151,18 +152,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
   auto store_o = [&](int b, int hq, int d, float x) {
     reinterpret_cast<uint16_t*>(p.o)[b * p.o_sb + hq * p.o_sh + d] = p.o_bf16 ? from_f32<true>(x) : from_f32<false>(x);
   };
-  // after a wait has given up on this device, here or in an earlier launch, the caller gets NaN and no stale memory
-  if (cta_device_failed()) {
-    const float nan = __int_as_float(0x7fc00000);
-    const long long rows = static_cast<long long>(p.batch) * p.hq;
-    for (long long i = blockIdx.x * static_cast<long long>(NTHR) + tid; i < rows * D; i += static_cast<long long>(gridDim.x) * NTHR) {
-      const long long row = i / D;
-      store_o(static_cast<int>(row / p.hq), static_cast<int>(row % p.hq), static_cast<int>(i % D), nan);
-      if (p.lse && i % D == 0) p.lse[row] = nan;
-    }
-    return;
-  }
-  // aligned by an offset: a pointer that went through an integer would be loaded from with generic instructions
+  const bool gave_up = device_failed();   // asked for here, answered at the first barrier
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((0u - smem_u32(smem_raw)) & 1023u);
   const uint32_t sbase = smem_u32(smem);
@@ -201,7 +191,18 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
       fence_proxy_async();
     }
   }
-  __syncthreads();
+  // after a wait has given up on this device, here or in an earlier launch, the caller gets NaN and no stale memory
+  if (__syncthreads_or(gave_up)) {
+    const float nan = __int_as_float(0x7fc00000);
+    const long long rows = static_cast<long long>(p.batch) * p.hq;
+    for (long long i = blockIdx.x * static_cast<long long>(NTHR) + tid; i < rows * D; i += static_cast<long long>(gridDim.x) * NTHR) {
+      const long long row = i / D;
+      store_o(static_cast<int>(row / p.hq), static_cast<int>(row % p.hq), static_cast<int>(i % D), nan);
+      if (p.lse && i % D == 0) p.lse[row] = nan;
+    }
+    return;
+  }
+  // aligned by an offset: a pointer that went through an integer would be loaded from with generic instructions
   // the host has checked that all tiles of a call fit 31 bits
   const int total = pre[p.batch] * hkv;
   const int per = max((total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x), W);
@@ -401,17 +402,33 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
             const int d = kk * 16 + 2 * t + 8 * r;
-            qb[nt][kk][r] = head < p.groups ? static_cast<uint32_t>(src[d]) | (static_cast<uint32_t>(src[d + 1]) << 16) : 0u;
+            qb[nt][kk][r] = head >= p.groups ? 0u
+                            : p.q_align >= 4 ? *reinterpret_cast<const uint32_t*>(src + d)
+                                             : static_cast<uint32_t>(src[d]) | (static_cast<uint32_t>(src[d + 1]) << 16);
           }
         cs[nt][0] = cs[nt][1] = p.scale_log2;
       } else {
         float f[D / 4], top = 0.0f;
+        // the lane's channels in the order in which their codes are taken from shared memory: D / 4 in a row
+        uint32_t v[D / 8];
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+          const uint16_t* at = src + t * (D / 4) + 8 * i;
+          uint4 x = make_uint4(0, 0, 0, 0);
+          if (head < p.groups) {
+            if (p.q_align >= 16) {
+              x = *reinterpret_cast<const uint4*>(at);
+            } else {
+              x.x = at[0] | (static_cast<uint32_t>(at[1]) << 16); x.y = at[2] | (static_cast<uint32_t>(at[3]) << 16);
+              x.z = at[4] | (static_cast<uint32_t>(at[5]) << 16); x.w = at[6] | (static_cast<uint32_t>(at[7]) << 16);
+            }
+          }
+          v[4 * i] = x.x; v[4 * i + 1] = x.y; v[4 * i + 2] = x.z; v[4 * i + 3] = x.w;
+        }
 #pragma unroll
         for (int i = 0; i < D / 4; ++i) {
-          // the lane's i-th channel in the order in which its codes are taken from shared memory
-          const int d = FMT == kKvInt4 ? t * (D / 4) + i : (D == 128 ? (2 * t + i / 16) * 16 + i % 16 : t * 16 + i);
-          const uint16_t v = head < p.groups ? src[d] : static_cast<uint16_t>(0);
-          f[i] = p.q_bf16 ? to_f32<true>(v) : to_f32<false>(v);
+          const uint16_t w = static_cast<uint16_t>(i & 1 ? v[i / 2] >> 16 : v[i / 2] & 0xffffu);
+          f[i] = p.q_bf16 ? to_f32<true>(w) : to_f32<false>(w);
           top = fmaxf(top, fabsf(f[i]));
           if (f[i] != f[i]) top = INFINITY;
         }
@@ -772,44 +789,70 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     }
   }
 
-  // ---- pieces of one segment are joined, warps in order
+  // ---- pieces of one segment are joined, warps in order.  First the factors, a warp for each head and a lane for each piece;
+  // pieces of one segment are neighbours among those there are: the last pieces of some warps, then perhaps a first piece
   __syncthreads();
   const bool failed = *cta_abort != 0;
-  for (int e0 = 0; e0 < 2 * W;) {
-    const int seg = seg_of[e0];
-    if (seg < 0) { ++e0; continue; }
-    int e1 = e0 + 1;
-    while (e1 < 2 * W && (seg_of[e1] < 0 || seg_of[e1] == seg)) ++e1;
-    const int sb = seg / hkv, h = seg % hkv, n = pre[sb + 1] - pre[sb], first = pre[sb] * hkv + h * n;
-    const bool inside = first >= x0 && first + n <= x1;
-    const long long part = (static_cast<long long>(blockIdx.x) + seg) * p.groups;
-    for (int i = tid; i < p.groups * D; i += NTHR) {
-      const int head = i / D, d = i % D;
-      float top = -INFINITY, den = 0.0f, acc = 0.0f;
-      for (int e = e0; e < e1; ++e)
-        if (seg_of[e] >= 0) top = fmaxf(top, ml[e * H + head]);
-      for (int e = e0; e < e1; ++e) {
-        if (seg_of[e] < 0) continue;
-        const float mw = ml[e * H + head], lw = ml[(2 * W + e) * H + head];
-        if (lw == 0.0f) continue;
-        const float* from = (e & 1) ? reinterpret_cast<const float*>(smem + (e >> 1) * C::kRingWarp)
-                                    : p.piece_o + (static_cast<long long>(blockIdx.x) * W + (e >> 1)) * p.groups * D;
-        const float f = ex2_approx(mw == -INFINITY ? 0.0f : mw - top);
-        den += f * lw;
-        acc += f * from[i];
-      }
-      float val = den != 0.0f ? acc / den : 0.0f;
-      float lse = den != 0.0f ? log2f(den) - 14.0f + (top == -INFINITY ? 0.0f : top) : -INFINITY;
-      if (failed) val = lse = __int_as_float(0x7fc00000);
-      if (inside) {
-        store_o(sb, h * p.groups + head, d, val);
-        if (d == 0 && p.lse) p.lse[static_cast<long long>(sb) * p.hq + h * p.groups + head] = lse;
-      } else {
-        p.part_o[(part + head) * D + d] = val;
-        if (d == 0) p.part_lse[part + head] = lse;
-      }
+  const int piece_seg = lane < 2 * W ? seg_of[lane] : -1;
+  const uint32_t mates = __match_any_sync(0xffffffffu, piece_seg);
+  const bool leads = piece_seg >= 0 && (mates & ((1u << lane) - 1u)) == 0u;
+  const uint32_t leaders = __ballot_sync(0xffffffffu, leads);
+  if (leaders == 0u) return;
+  for (int head = warp; head < p.groups; head += W) {
+    const bool on = piece_seg >= 0;
+    const float mine = on ? ml[lane * H + head] : -INFINITY, sum = on ? ml[(2 * W + lane) * H + head] : 0.0f;
+    float top = -INFINITY, den = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 2 * W; ++e) {
+      const float x = __shfl_sync(0xffffffffu, mine, e);
+      if ((mates >> e) & 1u) top = fmaxf(top, x);
     }
-    e0 = e1;
+    // (a NaN sum has no maximum of its own)
+    const float f = sum != 0.0f ? ex2_approx(mine == -INFINITY ? 0.0f : mine - top) : 0.0f;
+    const float share_of = f * sum;
+#pragma unroll
+    for (int e = 0; e < 2 * W; ++e) {
+      const float x = __shfl_sync(0xffffffffu, share_of, e);
+      if ((mates >> e) & 1u) den += x;
+    }
+    if (on) {
+      ml[lane * H + head] = den != 0.0f ? f / den : 0.0f;
+      ml[(2 * W + lane) * H + head] = den != 0.0f ? log2f(den) - 14.0f + (top == -INFINITY ? 0.0f : top) : -INFINITY;
+    }
+  }
+  __syncthreads();
+  const int chains = __popc(leaders);
+  for (int i = tid; i < chains * p.groups * (D / 4); i += NTHR) {
+    const int chain = i / (p.groups * (D / 4)), rest = i - chain * (p.groups * (D / 4)), head = rest / (D / 4), d = rest % (D / 4) * 4;
+    uint32_t from = leaders;
+    for (int c = 0; c < chain; ++c) from &= from - 1u;
+    const int e0 = __ffs(from) - 1, seg = seg_of[e0];
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+    for (int e = e0; e < 2 * W; ++e) {
+      const int es = seg_of[e];
+      if (es < 0) continue;
+      if (es != seg) break;
+      const float f = ml[e * H + head];
+      if (f == 0.0f) continue;   // nothing of the piece was stored, perhaps
+      const float4 x = *reinterpret_cast<const float4*>(
+          ((e & 1) ? reinterpret_cast<const float*>(smem + (e >> 1) * C::kRingWarp)
+                   : p.piece_o + (static_cast<long long>(blockIdx.x) * W + (e >> 1)) * p.groups * D) + head * D + d);
+      acc.x += f * x.x; acc.y += f * x.y; acc.z += f * x.z; acc.w += f * x.w;
+    }
+    float lse = ml[(2 * W + e0) * H + head];
+    if (failed) acc.x = acc.y = acc.z = acc.w = lse = __int_as_float(0x7fc00000);
+    const int sb = seg / hkv, h = seg % hkv, n = pre[sb + 1] - pre[sb], first = pre[sb] * hkv + h * n;
+    if (first >= x0 && first + n <= x1) {
+      uint16_t* row = reinterpret_cast<uint16_t*>(p.o) + sb * p.o_sb + static_cast<long long>(h * p.groups + head) * p.o_sh + d;
+      reinterpret_cast<uint32_t*>(row)[0] = p.o_bf16 ? pack_bf16x2(acc.x, acc.y) : pack_f16x2(acc.x, acc.y);
+      reinterpret_cast<uint32_t*>(row)[1] = p.o_bf16 ? pack_bf16x2(acc.z, acc.w) : pack_f16x2(acc.z, acc.w);
+      if (d == 0 && p.lse) p.lse[static_cast<long long>(sb) * p.hq + h * p.groups + head] = lse;
+    } else {
+      const long long part = (static_cast<long long>(blockIdx.x) + seg) * p.groups + head;
+      *reinterpret_cast<float4*>(p.part_o + part * D + d) = acc;
+      if (d == 0) p.part_lse[part] = lse;
+    }
   }
 }
 

@@ -1443,6 +1443,8 @@ int sqattn_paged_decode(const sqattn_paged_decode_args* a, sqattn_stream_t strea
   p.lse = a->lse; p.kv_lens = a->kv_lens; p.list = a->pages; p.list_len = a->num_listed;
   p.max_len = pl.max_len;
   p.batch = a->batch; p.hq = a->num_q_heads; p.groups = a->num_q_heads / pool->num_kv_heads;
+  const uintptr_t q_bits = reinterpret_cast<uintptr_t>(a->q.ptr) | static_cast<uintptr_t>(a->q.stride_b * 2) | static_cast<uintptr_t>(a->q.stride_h * 2);
+  p.q_align = q_bits % 16 == 0 ? 16 : q_bits % 4 == 0 ? 4 : 2;
   p.q_bf16 = pool->dtype == SQATTN_BF16; p.o_bf16 = a->o_dtype == SQATTN_BF16;
   const double scale = a->sm_scale > 0.0f ? static_cast<double>(a->sm_scale) : 1.0 / sqrt(static_cast<double>(pool->head_dim));
   p.scale_log2 = std::max(static_cast<float>(scale * 1.4426950408889634), 1e-30f);   // a factor of 0 would turn masked scores into NaN

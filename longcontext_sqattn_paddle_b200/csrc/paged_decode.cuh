@@ -54,7 +54,7 @@ struct PagedDecodeParams {
   float scale_log2;  // softmax scale * log2(e)
   float* part_o;     // [grid + B * Hkv, groups, D] fp32, each divided by its own sum
   float* part_lse;   // [grid + B * Hkv, groups]
-  float* piece_o;    // [grid * warps, groups, D] fp32: what a warp's first segment has of it, if that ends inside the stretch
+  float* piece_o;    // [grid * warps, 8 or 16 columns, D] fp32: what a warp's first segment has of it, if that ends inside the stretch
   int* plan;         // [B + 2]: tiles per KV head before each sequence, then tiles per CTA
   int* cut;          // [grid]: segment that begins in the CTA before and goes on in this one, or -1
 };
@@ -745,27 +745,25 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
       // a piece: the last one of the stretch into the ring, which is empty by then, one before it to global scratch
       const bool last = seg_end == xw1 || !ok;
       const int slot = warp * 2 + (last ? 1 : 0);
-      float* to = last ? reinterpret_cast<float*>(smem + warp * C::kRingWarp)
-                       : p.piece_o + (static_cast<long long>(blockIdx.x) * W + warp) * p.groups * D;
+      // in the order of the products' results, 16 bytes a lane: by rows of the output the stores would fall on two banks
+      float4* to = reinterpret_cast<float4*>(last ? reinterpret_cast<float*>(smem + warp * C::kRingWarp)
+                                                  : p.piece_o + (static_cast<long long>(blockIdx.x) * W + warp) * (H * D)) + lane;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      for (int nt = 0; nt < NT; ++nt) {
+        if (ok) {
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const int col = nt * 8 + 2 * t + c;
-          if (col < p.groups) {
-            if (ok) {
+          for (int i = 0; i < D / 16; ++i)
+            to[(nt * (D / 16) + i) * 32] = make_float4(o[nt][i][0] * unit, o[nt][i][1] * unit, o[nt][i][2] * unit, o[nt][i][3] * unit);
+        }
+        if (g == 0) {
 #pragma unroll
-              for (int i = 0; i < D / 16; ++i) {
-                to[col * D + channel(i, 0)] = o[nt][i][c] * unit;
-                to[col * D + channel(i, 2)] = o[nt][i][c + 2] * unit;
-              }
-            }
-            if (g == 0) {
-              ml[slot * H + col] = m[nt][c];
-              ml[(2 * W + slot) * H + col] = l[nt][c];
-            }
+          for (int c = 0; c < 2; ++c) {
+            const int col = nt * 8 + 2 * t + c;
+            ml[slot * H + col] = m[nt][c];
+            ml[(2 * W + slot) * H + col] = l[nt][c];
           }
         }
+      }
       if (lane == 0) seg_of[slot] = b * hkv + h;
     }
     if (!ok) break;
@@ -798,7 +796,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
   const bool leads = piece_seg >= 0 && (mates & ((1u << lane) - 1u)) == 0u;
   const uint32_t leaders = __ballot_sync(0xffffffffu, leads);
   if (leaders == 0u) return;
-  for (int head = warp; head < p.groups; head += W) {
+  for (int head = warp; head < H; head += W) {   // unused columns, too: they are read in pairs
     const bool on = piece_seg >= 0;
     const float mine = on ? ml[lane * H + head] : -INFINITY, sum = on ? ml[(2 * W + lane) * H + head] : 0.0f;
     float top = -INFINITY, den = 0.0f;
@@ -821,37 +819,46 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     }
   }
   __syncthreads();
+  // then the sums, in the order in which the pieces lie: four of a lane's results at a time
   const int chains = __popc(leaders);
-  for (int i = tid; i < chains * p.groups * (D / 4); i += NTHR) {
-    const int chain = i / (p.groups * (D / 4)), rest = i - chain * (p.groups * (D / 4)), head = rest / (D / 4), d = rest % (D / 4) * 4;
+  for (int i = tid; i < chains * (H * D / 4); i += NTHR) {
+    const int chain = i / (H * D / 4), at = i % (H * D / 4), nt = at / (D / 16 * 32), fi = at / 32 % (D / 16), fl = at % 32;
+    const int col = nt * 8 + 2 * (fl & 3);
+    if (col >= p.groups) continue;
     uint32_t from = leaders;
     for (int c = 0; c < chain; ++c) from &= from - 1u;
     const int e0 = __ffs(from) - 1, seg = seg_of[e0];
     float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
     for (int e = e0; e < 2 * W; ++e) {
       const int es = seg_of[e];
       if (es < 0) continue;
       if (es != seg) break;
-      const float f = ml[e * H + head];
-      if (f == 0.0f) continue;   // nothing of the piece was stored, perhaps
-      const float4 x = *reinterpret_cast<const float4*>(
-          ((e & 1) ? reinterpret_cast<const float*>(smem + (e >> 1) * C::kRingWarp)
-                   : p.piece_o + (static_cast<long long>(blockIdx.x) * W + (e >> 1)) * p.groups * D) + head * D + d);
-      acc.x += f * x.x; acc.y += f * x.y; acc.z += f * x.z; acc.w += f * x.w;
+      const float2 f = *reinterpret_cast<const float2*>(ml + e * H + col);
+      if (f.x == 0.0f && f.y == 0.0f) continue;   // nothing of the piece was stored, perhaps
+      const float4 x = reinterpret_cast<const float4*>((e & 1) ? reinterpret_cast<const float*>(smem + (e >> 1) * C::kRingWarp)
+                                                               : p.piece_o + (static_cast<long long>(blockIdx.x) * W + (e >> 1)) * (H * D))[at];
+      acc.x += f.x * x.x; acc.y += f.y * x.y; acc.z += f.x * x.z; acc.w += f.y * x.w;
     }
-    float lse = ml[(2 * W + e0) * H + head];
-    if (failed) acc.x = acc.y = acc.z = acc.w = lse = __int_as_float(0x7fc00000);
+    float2 lse = *reinterpret_cast<const float2*>(ml + (2 * W + e0) * H + col);
+    if (failed) acc.x = acc.y = acc.z = acc.w = lse.x = lse.y = __int_as_float(0x7fc00000);
     const int sb = seg / hkv, h = seg % hkv, n = pre[sb + 1] - pre[sb], first = pre[sb] * hkv + h * n;
-    if (first >= x0 && first + n <= x1) {
-      uint16_t* row = reinterpret_cast<uint16_t*>(p.o) + sb * p.o_sb + static_cast<long long>(h * p.groups + head) * p.o_sh + d;
-      reinterpret_cast<uint32_t*>(row)[0] = p.o_bf16 ? pack_bf16x2(acc.x, acc.y) : pack_f16x2(acc.x, acc.y);
-      reinterpret_cast<uint32_t*>(row)[1] = p.o_bf16 ? pack_bf16x2(acc.z, acc.w) : pack_f16x2(acc.z, acc.w);
-      if (d == 0 && p.lse) p.lse[static_cast<long long>(sb) * p.hq + h * p.groups + head] = lse;
-    } else {
-      const long long part = (static_cast<long long>(blockIdx.x) + seg) * p.groups + head;
-      *reinterpret_cast<float4*>(p.part_o + part * D + d) = acc;
-      if (d == 0) p.part_lse[part] = lse;
+    const bool inside = first >= x0 && first + n <= x1;
+    const int fg = fl >> 2, d0 = kNative ? 16 * fi + fg : (D / 8) * fg + 2 * fi, d1 = kNative ? d0 + 8 : d0 + 1;
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      if (col + c >= p.groups) break;
+      const float a0 = c ? acc.y : acc.x, a1 = c ? acc.w : acc.z, l1 = c ? lse.y : lse.x;
+      const int hq = h * p.groups + col + c;
+      if (inside) {
+        store_o(sb, hq, d0, a0);
+        store_o(sb, hq, d1, a1);
+        if (at % (D / 16 * 32) < 4 && p.lse) p.lse[static_cast<long long>(sb) * p.hq + hq] = l1;
+      } else {
+        const long long part = (static_cast<long long>(blockIdx.x) + seg) * p.groups + col + c;
+        p.part_o[part * D + d0] = a0;
+        p.part_o[part * D + d1] = a1;
+        if (at % (D / 16 * 32) < 4) p.part_lse[part] = l1;
+      }
     }
   }
 }

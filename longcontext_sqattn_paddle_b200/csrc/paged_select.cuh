@@ -59,17 +59,17 @@ __global__ void __launch_bounds__(256) paged_score_kernel(const __grid_constant_
   __shared__ double u_s[D];
   griddep_launch();
   const int h = blockIdx.y, b = blockIdx.z;
-  const int held = held_pages(p, b);
-  if (held <= p.budget || static_cast<int>(blockIdx.x) * kPer >= held) return;   // all of them are taken: nothing to score
   const int grp = threadIdx.x / kLanes, c = threadIdx.x % kLanes;
   const int first = blockIdx.x * kPer + grp;
   uint4 lo[kScorePages], hi[kScorePages];
   int page[kScorePages];
 #pragma unroll
-  for (int j = 0; j < kScorePages; ++j) {
-    const int i = first + j * (256 / kLanes);
-    page[j] = i < held ? page_of(p.table, b, i, p.pool.num_pages) : -1;
-  }
+  for (int j = 0; j < kScorePages; ++j) page[j] = page_of(p.table, b, first + j * (256 / kLanes), p.pool.num_pages);   // beside the length
+  const int held = held_pages(p, b);
+  if (held <= p.budget || static_cast<int>(blockIdx.x) * kPer >= held) return;   // all of them are taken: nothing to score
+#pragma unroll
+  for (int j = 0; j < kScorePages; ++j)
+    if (first + j * (256 / kLanes) >= held) page[j] = -1;
 #pragma unroll
   for (int j = 0; j < kScorePages; ++j) {
     lo[j] = hi[j] = make_uint4(0, 0, 0, 0);
@@ -115,6 +115,8 @@ __global__ void __launch_bounds__(256) paged_score_kernel(const __grid_constant_
 }
 
 constexpr int kPickBins = 2048;
+constexpr int kPickKeys = 16;                    // keys of a thread
+constexpr int kPickChunk = 1024 * kPickKeys;     // keys of a CTA at a time
 
 // exclusive sum over the CTA's 1024 threads in thread order; `total` is everyone's sum.  Ends with a barrier.
 __device__ __forceinline__ int cta_exclusive_sum(int x, int* scratch, int& total) {
@@ -139,12 +141,34 @@ __device__ __forceinline__ int cta_exclusive_sum(int x, int* scratch, int& total
   return before + inc - x;
 }
 
+// Places, in ascending order of the keys' indexes, of the marked keys of a chunk: key j of thread t has index 1024 j + t, so
+// counts go by j and warp.  Afterwards counts[32 j + warp] marked keys come before those of this warp with that j; returns the
+// number marked.
+__device__ __forceinline__ int chunk_counts(unsigned marked, int* counts, int* scratch) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int j = 0; j < kPickKeys; ++j) {
+    const unsigned votes = __ballot_sync(0xffffffffu, (marked >> j) & 1u);
+    if (lane == 0) counts[j * 32 + warp] = __popc(votes);
+  }
+  __syncthreads();
+  int total;
+  const int mine = threadIdx.x < kPickKeys * 32 ? counts[threadIdx.x] : 0;
+  const int before = cta_exclusive_sum(mine, scratch, total);
+  if (threadIdx.x < kPickKeys * 32) counts[threadIdx.x] = before;
+  __syncthreads();
+  return total;
+}
+__device__ __forceinline__ int chunk_place(unsigned marked, int j, const int* counts) {
+  const unsigned votes = __ballot_sync(0xffffffffu, (marked >> j) & 1u);
+  return counts[j * 32 + (threadIdx.x >> 5)] + __popc(votes & ((1u << (threadIdx.x & 31)) - 1u));
+}
+
 // One CTA per (KV head, sequence).  The budget-th highest key is found by histograms: 2048 equal bins over the range of the
 // keys still in question, then over the bin that the budget ends in, until that bin holds no more keys than are wanted or one
-// value only (two rounds for scores as they occur, six at most).  A thread takes 16 consecutive keys at a time, so that one
-// sum over the CTA gives the ascending list; keys are read again in every round, from L1 up to 16384 pages.
+// value only (two rounds for scores as they occur, six at most).  Up to 16384 pages the keys stay in registers; more are read
+// again in every round.
 __global__ void __launch_bounds__(1024) paged_pick_kernel(const __grid_constant__ PagedSelectParams p) {
-  constexpr int kRun = 16;
   __shared__ int hist[kPickBins], scratch[32], found[3];
   __shared__ unsigned long long red[2][32];
   griddep_launch();
@@ -159,18 +183,28 @@ __global__ void __launch_bounds__(1024) paged_pick_kernel(const __grid_constant_
   }
   // pages that are taken without a score (sink + recent <= budget < held, so the two do not meet)
   const int lo_i = p.sink_pages, hi_i = held - p.recent_pages;
+  const bool many = held > kPickChunk;
+  unsigned long long k[kPickKeys];
+  unsigned in = 0;  // which of them are in the running
+  auto load = [&](int i0) {
+    in = 0;
+#pragma unroll
+    for (int j = 0; j < kPickKeys; ++j) {
+      const int i = i0 + j * 1024 + tid;
+      const bool on = i >= lo_i && i < hi_i;
+      k[j] = on ? keys[i] : 0ull;
+      in |= static_cast<unsigned>(on) << j;
+    }
+  };
+  load(0);
   int want = p.budget - p.sink_pages - p.recent_pages;
   unsigned long long lo = ~0ull, hi = 0ull;
-  for (int i0 = 0; i0 < held; i0 += 1024 * kRun)
+  for (int i0 = 0; i0 < held; i0 += kPickChunk) {
+    if (i0 > 0) load(i0);
 #pragma unroll
-    for (int j = 0; j < kRun; ++j) {
-      const int i = i0 + tid * kRun + j;
-      if (i >= lo_i && i < hi_i) {
-        const unsigned long long k = keys[i];
-        lo = min(lo, k);
-        hi = max(hi, k);
-      }
-    }
+    for (int j = 0; j < kPickKeys; ++j)
+      if ((in >> j) & 1u) { lo = min(lo, k[j]); hi = max(hi, k[j]); }
+  }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     lo = min(lo, __shfl_xor_sync(0xffffffffu, lo, o));
@@ -178,8 +212,13 @@ __global__ void __launch_bounds__(1024) paged_pick_kernel(const __grid_constant_
   }
   if (lane == 0) { red[0][warp] = lo; red[1][warp] = hi; }
   __syncthreads();
+  lo = red[0][lane];
+  hi = red[1][lane];
 #pragma unroll
-  for (int w = 0; w < 32; ++w) { lo = min(lo, red[0][w]); hi = max(hi, red[1][w]); }
+  for (int o = 16; o > 0; o >>= 1) {
+    lo = min(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+    hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+  }
   // keys above `hi` are taken, keys below `lo` are not, `want` of those between are.  (hi < ~0: no score has that key.)
   unsigned long long from = hi + 1ull;  // what is taken without a look at its place
   while (want > 0) {
@@ -187,15 +226,12 @@ __global__ void __launch_bounds__(1024) paged_pick_kernel(const __grid_constant_
     const int shift = max(0, 53 - __clzll(span));  // (hi - lo) >> shift < 2048
     hist[tid] = hist[1024 + tid] = 0;
     __syncthreads();
-    for (int i0 = 0; i0 < held; i0 += 1024 * kRun)
+    for (int i0 = 0; i0 < held; i0 += kPickChunk) {
+      if (many) load(i0);
 #pragma unroll
-      for (int j = 0; j < kRun; ++j) {
-        const int i = i0 + tid * kRun + j;
-        if (i >= lo_i && i < hi_i) {
-          const unsigned long long k = keys[i];
-          if (k >= lo && k <= hi) atomicAdd(&hist[static_cast<int>((k - lo) >> shift)], 1);
-        }
-      }
+      for (int j = 0; j < kPickKeys; ++j)
+        if (((in >> j) & 1u) && k[j] >= lo && k[j] <= hi) atomicAdd(&hist[static_cast<int>((k[j] - lo) >> shift)], 1);
+    }
     __syncthreads();
     // from the highest bin down: thread t has bins 2047 - 2 t and 2046 - 2 t
     const int b0 = kPickBins - 1 - 2 * tid, n0 = hist[b0], n1 = hist[b0 - 1];
@@ -220,29 +256,38 @@ __global__ void __launch_bounds__(1024) paged_pick_kernel(const __grid_constant_
     if (lo == hi) break;                                 // one value: the lowest pages of it
     __syncthreads();
   }
+  __syncthreads();
   int taken = 0, ties = 0;  // before this chunk
-  for (int i0 = 0; i0 < held; i0 += 1024 * kRun) {
+  for (int i0 = 0; i0 < held; i0 += kPickChunk) {
+    if (many) load(i0);
     unsigned take = 0, tie = 0;
 #pragma unroll
-    for (int j = 0; j < kRun; ++j) {
-      const int i = i0 + tid * kRun + j;
-      if (i >= held) continue;
-      const bool always = i < lo_i || i >= hi_i;
-      const unsigned long long k = always ? 0ull : keys[i];
-      if (always || k >= from) take |= 1u << j;
-      else if (want > 0 && k == lo) tie |= 1u << j;
+    for (int j = 0; j < kPickKeys; ++j) {
+      const int i = i0 + j * 1024 + tid;
+      const bool on = (in >> j) & 1u;
+      if (i < held && (!on || k[j] >= from)) take |= 1u << j;
+      else if (on && k[j] == lo) tie |= 1u << j;
     }
-    int all;
-    const int tie_at = ties + cta_exclusive_sum(__popc(tie), scratch, all);
-    ties += all;
-    for (int room = want - tie_at; tie && room > 0; --room) {  // the lowest of this thread's ties that there is room for
-      const unsigned low = tie & (0u - tie);
-      take |= low;
-      tie ^= low;
+    if (want > 0) {   // of the keys equal to lo the first `want`
+      const int n = chunk_counts(tie, hist, scratch);
+      unsigned more = 0;
+#pragma unroll
+      for (int j = 0; j < kPickKeys; ++j) {
+        const int place = chunk_place(tie, j, hist);
+        if (((tie >> j) & 1u) && ties + place < want) more |= 1u << j;
+      }
+      take |= more;
+      ties += n;
+      __syncthreads();
     }
-    int at = taken + cta_exclusive_sum(__popc(take), scratch, all);
-    taken += all;
-    for (; take; take &= take - 1) out[at++] = i0 + tid * kRun + __ffs(take) - 1;
+    const int n = chunk_counts(take, hist, scratch);
+#pragma unroll
+    for (int j = 0; j < kPickKeys; ++j) {
+      const int place = chunk_place(take, j, hist);
+      if ((take >> j) & 1u) out[taken + place] = i0 + j * 1024 + tid;
+    }
+    taken += n;
+    __syncthreads();
   }
 }
 

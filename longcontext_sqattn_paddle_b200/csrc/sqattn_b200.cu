@@ -650,7 +650,7 @@ int plan_paged_decode(const sqattn_paged_decode_args* a, PagedDecodePlan* pl) {
   const size_t parts = static_cast<size_t>(pl->grid) + static_cast<size_t>(a->batch) * pool->num_kv_heads;
   pl->lse_off = align_up(parts * row, 256);
   pl->piece_off = pl->lse_off + align_up(parts * groups * 4, 256);
-  pl->plan_off = pl->piece_off + align_up(static_cast<size_t>(pl->grid) * warps * row, 256);
+  pl->plan_off = pl->piece_off + align_up(static_cast<size_t>(pl->grid) * warps * (groups > 8 ? 16 : 8) * pool->head_dim * 4, 256);
   pl->cut_off = pl->plan_off + align_up((static_cast<size_t>(a->batch) + 2) * 4, 256);
   pl->total = pl->cut_off + align_up(static_cast<size_t>(pl->grid) * 4, 256);
   return SQATTN_OK;

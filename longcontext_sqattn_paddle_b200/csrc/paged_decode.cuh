@@ -36,6 +36,8 @@
 namespace sq {
 
 constexpr int kPagedMaxBatch = 1024;
+constexpr int kPagedCluster = 8;
+constexpr int kPagedMaxClusters = 16;  // two to a GPC
 
 struct PagedDecodeParams {
   PagedPool pool;
@@ -50,6 +52,7 @@ struct PagedDecodeParams {
   int list_len;
   int max_len;  // what the table, or the caller's bound, holds
   int batch, hq, groups, q_bf16, o_bf16;
+  int clusters;      // a cluster of kPagedCluster CTAs for each segment: they join its parts themselves
   int q_align;       // bytes that every head's row is aligned to: 16, 4 or 2
   float scale_log2;  // softmax scale * log2(e)
   float* part_o;     // [grid + B * Hkv, groups, D] fp32, each divided by its own sum
@@ -62,9 +65,12 @@ struct PagedDecodeParams {
 template <int FMT, int D, int NT>
 struct PagedDecodeCfg {
   static constexpr int kRow = kv_row_bytes<FMT>(D);
+  // Measured (us; 1M native | 16 ragged int8 | 512K int4, 28/4 and 32/8 heads): native 8 warps of one tile in flight 319, 4 of two
+  // 321, of three 338-351; int8 8 of two 131, 10 137, 12 147, 6 149; int4 12 warps of two 64-key tiles 68, of two 32-key tiles 75,
+  // 16 of two 32-key tiles 84, 8 86.  More than about 130 KB in flight an SM is slower, whatever holds it.
   static constexpr int kTile = FMT == kKvInt4 ? 64 : 32;                 // keys of a tile
-  static constexpr int kWarps = FMT == kKvNative ? (D == 128 ? 4 : 8) : (NT == 2 ? 8 : 12);
-  static constexpr int kStages = 2;
+  static constexpr int kWarps = FMT == kKvInt4 && NT == 1 ? 12 : 8;
+  static constexpr int kStages = FMT == kKvNative && D == 128 ? 1 : 2;   // tiles a warp has in flight
   static constexpr int kTensor = kTile * kRow;                           // a tile's keys or values
   static constexpr int kRingWarp = kStages * 2 * kTensor;
   static constexpr int kScaleOff = kWarps * kRingWarp;                   // [warp][stage][K, V][kTile] fp32
@@ -76,8 +82,9 @@ struct PagedDecodeCfg {
   static constexpr int kSegOff = kRecOff + kWarps * 32 * 32;             // [2 warps] segments of the pieces
   static constexpr int kMiscOff = kSegOff + 2 * kWarps * 4;              // abort flag, exponents of codes
   static constexpr int kPlanOff = (kMiscOff + 16 + 15) / 16 * 16;        // [B + 1]
-  static constexpr int total(int batch) { return kPlanOff + (batch + 1) * 4 + 1024; }
-  static_assert(total(kPagedMaxBatch) <= 227 * 1024, "shared memory of a CTA");
+  __host__ __device__ static constexpr int share_off(int batch) { return (kPlanOff + (batch + 1) * 4 + 15) / 16 * 16; }  // clusters: a CTA's part [8 NT][D], LSE [8 NT]
+  __host__ __device__ static constexpr int total(int batch, bool clusters) { return share_off(batch) + (clusters ? 8 * NT * (D + 1) * 4 : 0) + 1024; }
+  static_assert(total(kPagedMaxBatch, false) <= 227 * 1024 && total(kPagedMaxClusters, true) <= 227 * 1024, "shared memory of a CTA");
   static_assert(8 * NT * D * 4 <= kRingWarp, "a warp's last piece takes the place of its ring");
 };
 
@@ -90,6 +97,25 @@ __device__ __forceinline__ void mma_16832_int(int (&c)[4], uint32_t a0, uint32_t
   else
     asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.u8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// every thread of the cluster, with its shared memory's writes; a thread that has ended counts as arrived
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t cluster_address(uint32_t local, int rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(local), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ float4 cluster_load4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ float2 cluster_load2(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+  return v;
 }
 __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t a) {
   uint32_t r;
@@ -200,15 +226,29 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
       store_o(static_cast<int>(row / p.hq), static_cast<int>(row % p.hq), static_cast<int>(i % D), nan);
       if (p.lse && i % D == 0) p.lse[row] = nan;
     }
+    if (p.clusters) {   // the others of the cluster may not have noticed: they find the failure in this CTA's part
+      float* part_lse = reinterpret_cast<float*>(smem + C::share_off(p.batch)) + H * D;
+      if (tid < H) part_lse[tid] = nan;
+      cluster_barrier();
+      cluster_barrier();
+    }
     return;
   }
   // aligned by an offset: a pointer that went through an integer would be loaded from with generic instructions
   // the host has checked that all tiles of a call fit 31 bits
   const int total = pre[p.batch] * hkv;
   const int per = max((total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x), W);
-  const long long cta_first = static_cast<long long>(blockIdx.x) * per;
-  const int x0 = static_cast<int>(min(cta_first, static_cast<long long>(total)));
-  const int x1 = static_cast<int>(min(cta_first + per, static_cast<long long>(total)));
+  int x0, x1;
+  if (p.clusters) {
+    const int seg = blockIdx.x / kPagedCluster, b = seg / hkv, n = pre[b + 1] - pre[b], mine = (n + kPagedCluster - 1) / kPagedCluster;
+    const int first = pre[b] * hkv + seg % hkv * n;
+    x0 = min(first + n, first + static_cast<int>(blockIdx.x % kPagedCluster) * mine);
+    x1 = min(first + n, x0 + mine);
+  } else {
+    const long long first = static_cast<long long>(blockIdx.x) * per;
+    x0 = static_cast<int>(min(first, static_cast<long long>(total)));
+    x1 = static_cast<int>(min(first + per, static_cast<long long>(total)));
+  }
 
   // sequence of tile x
   auto seq_of = [&](int x) {
@@ -219,11 +259,11 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     }
     return lo;
   };
-  if (blockIdx.x == 0) {
+  if (blockIdx.x == 0 && !p.clusters) {
     for (int b = tid; b <= p.batch; b += NTHR) p.plan[b] = pre[b];
     if (tid == 0) p.plan[p.batch + 1] = per;
   }
-  if (tid == 0) {
+  if (tid == 0 && !p.clusters) {
     int cut = -1;
     if (x0 > 0 && x0 < x1) {
       const int b = seq_of(x0), n = pre[b + 1] - pre[b], h = (x0 - pre[b] * hkv) / n, first = pre[b] * hkv + h * n;
@@ -238,7 +278,9 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         store_o(b, i / D, i % D, 0.0f);
         if (p.lse && i % D == 0) p.lse[static_cast<long long>(b) * p.hq + i / D] = -INFINITY;
       }
-  if (x0 >= x1) return;
+  float* share = reinterpret_cast<float*>(smem + C::share_off(p.batch));   // clusters: this CTA's part
+  if (p.clusters && tid < H) share[H * D + tid] = -INFINITY;
+  if (x0 < x1) {
   // this warp's tiles: xw0, xw0 + step, .. below xw1.  In a CTA whose tiles are all of one segment the warps take turns, so that
   // together they read neighbouring rows (1M tokens native: 348 us in stretches, 338 in turns)
   int xw0, xw1, step;
@@ -795,7 +837,6 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
   const uint32_t mates = __match_any_sync(0xffffffffu, piece_seg);
   const bool leads = piece_seg >= 0 && (mates & ((1u << lane) - 1u)) == 0u;
   const uint32_t leaders = __ballot_sync(0xffffffffu, leads);
-  if (leaders == 0u) return;
   for (int head = warp; head < H; head += W) {   // unused columns, too: they are read in pairs
     const bool on = piece_seg >= 0;
     const float mine = on ? ml[lane * H + head] : -INFINITY, sum = on ? ml[(2 * W + lane) * H + head] : 0.0f;
@@ -843,6 +884,11 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     if (failed) acc.x = acc.y = acc.z = acc.w = lse.x = lse.y = __int_as_float(0x7fc00000);
     const int sb = seg / hkv, h = seg % hkv, n = pre[sb + 1] - pre[sb], first = pre[sb] * hkv + h * n;
     const bool inside = first >= x0 && first + n <= x1;
+    if (p.clusters) {
+      reinterpret_cast<float4*>(share)[at] = acc;
+      if (at % (D / 16 * 32) < 4) { share[H * D + col] = lse.x; share[H * D + col + 1] = lse.y; }
+      continue;
+    }
     const int fg = fl >> 2, d0 = kNative ? 16 * fi + fg : (D / 8) * fg + 2 * fi, d1 = kNative ? d0 + 8 : d0 + 1;
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
@@ -861,6 +907,51 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
       }
     }
   }
+  }
+  if (!p.clusters) return;
+
+  // ---- a cluster's parts of one segment: every CTA joins an eighth of the columns' channels
+  cluster_barrier();
+  {
+    const int rank = blockIdx.x % kPagedCluster, seg = blockIdx.x / kPagedCluster, sb = seg / hkv, h = seg % hkv;
+    constexpr int kMine = H * D / 4 / kPagedCluster;
+    const uint32_t at_o = sbase + C::share_off(p.batch), at_lse = at_o + H * D * 4;
+    if (pre[sb + 1] > pre[sb])
+      for (int i = tid; i < kMine; i += NTHR) {
+        const int at = rank * kMine + i, nt = at / (D / 16 * 32), fi = at / 32 % (D / 16), fl = at % 32, col = nt * 8 + 2 * (fl & 3);
+        if (col >= p.groups) continue;
+        float2 lse[kPagedCluster], top = make_float2(-INFINITY, -INFINITY), den = make_float2(0.0f, 0.0f);
+        float4 x[kPagedCluster], acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int r = 0; r < kPagedCluster; ++r) {
+          lse[r] = cluster_load2(cluster_address(at_lse + col * 4, r));
+          x[r] = cluster_load4(cluster_address(at_o + at * 16, r));
+        }
+#pragma unroll
+        for (int r = 0; r < kPagedCluster; ++r) { top.x = fmaxf(top.x, lse[r].x); top.y = fmaxf(top.y, lse[r].y); }
+#pragma unroll
+        for (int r = 0; r < kPagedCluster; ++r) {
+          // a part without keys has an LSE of -inf and whatever the memory held
+          const float f0 = lse[r].x == -INFINITY ? 0.0f : ex2_approx(lse[r].x - top.x), f1 = lse[r].y == -INFINITY ? 0.0f : ex2_approx(lse[r].y - top.y);
+          if (f0 != 0.0f) { acc.x += f0 * x[r].x; acc.z += f0 * x[r].z; }
+          if (f1 != 0.0f) { acc.y += f1 * x[r].y; acc.w += f1 * x[r].w; }
+          den.x += f0;
+          den.y += f1;
+        }
+        const int fg = fl >> 2, d0 = kNative ? 16 * fi + fg : (D / 8) * fg + 2 * fi, d1 = kNative ? d0 + 8 : d0 + 1;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          if (col + c >= p.groups) break;
+          const float sum = c ? den.y : den.x, inv = sum != 0.0f ? 1.0f / sum : 0.0f;
+          const int hq = h * p.groups + col + c;
+          store_o(sb, hq, d0, (c ? acc.y : acc.x) * inv);
+          store_o(sb, hq, d1, (c ? acc.w : acc.z) * inv);
+          if (at % (D / 16 * 32) < 4 && p.lse)
+            p.lse[static_cast<long long>(sb) * p.hq + hq] = sum != 0.0f ? log2f(sum) + (c ? top.y : top.x) : -INFINITY;
+        }
+      }
+  }
+  cluster_barrier();   // nobody leaves while its shared memory is being read
 }
 
 // Joins the partial results of segments that lie in several CTAs.  Segment s = b * Hkv + h of tiles [first, last) has a part

@@ -443,7 +443,7 @@ class PagedPool:
     of every page's keys, None: not kept).  The format follows from the pages' type.  All tensors contiguous on one GPU."""
 
     __slots__ = ("k_pages", "v_pages", "k_scale", "v_scale", "k_bounds", "dtype", "kv_format", "num_pages", "num_kv_heads",
-                 "page_size", "head_dim", "device", "_struct", "_address")
+                 "page_size", "head_dim", "device", "device_index", "_struct", "_address", "_scratch")
 
     def __init__(self, k_pages, v_pages, k_scale=None, v_scale=None, k_bounds=None, dtype=None):
         kinds = {torch.int8: "int8", torch.uint8: "int4"}
@@ -477,6 +477,8 @@ class PagedPool:
         self._struct = L.PagedPool(*(0 if t is None else t.data_ptr() for t in (k_pages, v_pages, k_scale, v_scale, k_bounds)),
                                    self.num_pages, self.num_kv_heads, self.page_size, self.head_dim, code, L.KV_FORMAT[self.kv_format])
         self._address = C.addressof(self._struct)
+        self.device_index = self.device.index
+        self._scratch = {}   # workspace bytes of the calls' sizes
 
     @classmethod
     def allocate(cls, num_pages: int, page_size: int, num_kv_heads: int, head_dim: int, dtype=torch.bfloat16,
@@ -493,38 +495,71 @@ class PagedPool:
         return cls(*pages, *scales, k_bounds, dtype=dtype)
 
 
-def _paged_index(pool: PagedPool, block_table, batch: int, **ints):
-    """Check the index tensors of a paged call: int32, on the pool's device, one entry a sequence."""
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != batch or block_table.device != pool.device or \
-            (block_table.shape[1] > 1 and block_table.stride(1) != 1):
+# A CUDA tensor on the current device without the argument parser of torch.empty: 0.9 us against 2.4, of calls whose kernels take 3 to
+# 10.  (Inductor's allocation entry; torch.empty where a torch build has none.)
+_empty_strided = getattr(torch._C._dynamo.guards, "_empty_strided_cuda", None)
+
+
+def _paged_empty(pool: "PagedPool", shape, strides, dtype):
+    if _empty_strided is not None and torch._C._cuda_getDevice() == pool.device_index:
+        return _empty_strided(shape, strides, dtype)
+    return torch.empty_strided(shape, strides, dtype=dtype, device=pool.device)
+
+
+def _on_device(pool: PagedPool, call, *args):
+    """``call(*args, stream)`` with the pool's device current, on that device's current stream."""
+    index = pool.device_index
+    if torch._C._cuda_getDevice() == index:
+        code = call(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            code = call(*args, torch._C._cuda_getCurrentRawStream(index))
+    if code:
+        L.check(code)
+
+
+def _paged_table(pool: PagedPool, table, batch: int):
+    """Address, row stride and pages a sequence of a block table: int32 [batch, max_pages] with contiguous rows."""
+    shape, st = table.shape, table.stride()
+    if len(shape) != 2 or shape[0] != batch or table.dtype is not torch.int32 or table.get_device() != pool.device_index or \
+            (st[1] != 1 and shape[1] > 1):
         raise ValueError(f"block_table must be int32 [{batch}, max_pages] with contiguous rows on {pool.device}, got "
-                         f"{tuple(block_table.shape)} {block_table.dtype} on {block_table.device}")
-    for name, t in ints.items():
-        if t is not None and (t.dtype != torch.int32 or t.shape != (batch,) or t.device != pool.device or not t.is_contiguous()):
-            raise ValueError(f"{name} must be a contiguous int32 [{batch}] on {pool.device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
+                         f"{tuple(shape)} {table.dtype} on {table.device}")
+    return table.data_ptr(), st[0], shape[1]
+
+
+def _paged_ints(pool: PagedPool, t, batch: int, name: str) -> int:
+    """Address of a contiguous int32 [batch] on the pool's device."""
+    if t.dtype is not torch.int32 or t.shape != (batch,) or t.get_device() != pool.device_index or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 [{batch}] on {pool.device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
+    return t.data_ptr()
 
 
 def _paged_rows(pool: PagedPool, t, name: str):
     """New rows [B, N, Hkv, D] as the kernels read them: 16-byte pieces, copied only where the strides do not allow that."""
-    if t.dim() != 4 or t.shape[2] != pool.num_kv_heads or t.shape[3] != pool.head_dim or t.dtype != pool.dtype or t.device != pool.device:
+    shape = t.shape
+    if len(shape) != 4 or shape[2] != pool.num_kv_heads or shape[3] != pool.head_dim or t.dtype is not pool.dtype or \
+            t.get_device() != pool.device_index:
         raise ValueError(f"{name} must be [B, N, {pool.num_kv_heads}, {pool.head_dim}] {pool.dtype} on {pool.device}, got "
-                         f"{tuple(t.shape)} {t.dtype} on {t.device}")
+                         f"{tuple(shape)} {t.dtype} on {t.device}")
     st = t.stride()
-    if st[3] != 1 or t.data_ptr() % 16 or (st[0] | st[1] | st[2]) % 8:
+    if st[3] != 1 or (st[0] | st[1] | st[2]) % 8 or t.data_ptr() % 16:
         t = t.clone(memory_format=torch.contiguous_format)
-    return t
+        st = t.stride()
+    return t, L.Tensor(t.data_ptr(), st[0], st[2], st[1])
 
 
 def _paged_query(pool: PagedPool, q, layout: str):
-    """Descriptor and head count of a query [B, 1, Hq, D] (NHD) or [B, Hq, 1, D] (HND)."""
-    if q.dim() != 4 or q.dtype != pool.dtype or q.device != pool.device or q.shape[3] != pool.head_dim or q.stride(3) != 1:
-        raise ValueError(f"the query must have 4 dimensions, a contiguous last one of {pool.head_dim}, be {pool.dtype} and on {pool.device}, got "
-                         f"{tuple(q.shape)} {q.dtype} on {q.device}")
+    """Descriptor, batch and heads of a query [B, 1, Hq, D] (NHD) or [B, Hq, 1, D] (HND)."""
+    shape = q.shape
+    if len(shape) != 4 or q.dtype is not pool.dtype or q.get_device() != pool.device_index or shape[3] != pool.head_dim:
+        raise ValueError(f"the query must have 4 dimensions, the last of {pool.head_dim}, be {pool.dtype} and on {pool.device}, got "
+                         f"{tuple(shape)} {q.dtype} on {q.device}")
     desc = _desc(q, layout)
-    b, hq, one, _ = _shape(q, layout)
-    if one != 1:
-        raise ValueError(f"one query token a sequence, got {one}")
-    return desc, b, hq
+    tokens, hq = (shape[1], shape[2]) if layout == "NHD" else (shape[2], shape[1])
+    if tokens != 1:
+        raise ValueError(f"one query token a sequence, got {tokens}")
+    return desc, shape[0], hq
 
 
 def paged_write(pool: PagedPool, key, value, block_table, positions, counts=None) -> None:
@@ -533,40 +568,55 @@ def paged_write(pool: PagedPool, key, value, block_table, positions, counts=None
     ``counts[b]`` rows (int32 [B], None: all N).  Two sequences of one call must not write into the same page."""
     if key.shape != value.shape:
         raise ValueError(f"key and value must have one shape, got {tuple(key.shape)} and {tuple(value.shape)}")
-    key, value = _paged_rows(pool, key, "key"), _paged_rows(pool, value, "value")
+    key, kd = _paged_rows(pool, key, "key")
+    value, vd = _paged_rows(pool, value, "value")
     b, n = key.shape[:2]
-    _paged_index(pool, block_table, b, positions=positions, counts=counts)
-    if b == 0 or n == 0:
-        return
-    kd, vd = L.Tensor(*_desc(key, "NHD")), L.Tensor(*_desc(value, "NHD"))
-    with torch.cuda.device(pool.device):
-        L.check(L.lib.sqattn_paged_write(pool._address, C.addressof(kd), C.addressof(vd), b, n, block_table.data_ptr(), block_table.stride(0),
-                                         block_table.shape[1], positions.data_ptr(), None if counts is None else counts.data_ptr(), _stream()))
+    table, stride, pages = _paged_table(pool, block_table, b)
+    at = _paged_ints(pool, positions, b, "positions")
+    many = None if counts is None else _paged_ints(pool, counts, b, "counts")
+    if b and n:
+        _on_device(pool, L.lib.sqattn_paged_write, pool._address, C.addressof(kd), C.addressof(vd), b, n, table, stride, pages, at, many)
 
 
 def paged_read(pool: PagedPool, block_table, starts, num_rows: int, ends=None, out=None):
     """sqattn_paged_read: (key, value) [B, num_rows, Hkv, D] of positions ``starts[b] + i``, zeros at or past ``ends[b]``
     (int32 [B]; None: where the block table ends).  ``out``: a pair of tensors to write into (16-byte aligned rows)."""
     b = block_table.shape[0]
-    _paged_index(pool, block_table, b, starts=starts, ends=ends)
-    shape = (b, int(num_rows), pool.num_kv_heads, pool.head_dim)
+    table, stride, pages = _paged_table(pool, block_table, b)
+    at = _paged_ints(pool, starts, b, "starts")
+    until = None if ends is None else _paged_ints(pool, ends, b, "ends")
+    num_rows = int(num_rows)
+    hkv, d = pool.num_kv_heads, pool.head_dim
     if out is None:
-        out = tuple(torch.empty(shape, dtype=pool.dtype, device=pool.device) for _ in range(2))
+        shape, strides = (b, num_rows, hkv, d), (num_rows * hkv * d, hkv * d, d, 1)
+        out = _paged_empty(pool, shape, strides, pool.dtype), _paged_empty(pool, shape, strides, pool.dtype)
+        kd, vd = (L.Tensor(t.data_ptr(), strides[0], d, hkv * d) for t in out)
     else:
         for t in out:
             st = t.stride()
-            if t.shape != shape or t.dtype != pool.dtype or t.device != pool.device or st[3] != 1 or t.data_ptr() % 16 or (st[0] | st[1] | st[2]) % 8:
-                raise ValueError(f"out must be two {shape} {pool.dtype} tensors on {pool.device} with 16-byte aligned rows")
+            if t.shape != (b, num_rows, hkv, d) or t.dtype is not pool.dtype or t.get_device() != pool.device_index or st[3] != 1 or \
+                    t.data_ptr() % 16 or (st[0] | st[1] | st[2]) % 8:
+                raise ValueError(f"out must be two {(b, num_rows, hkv, d)} {pool.dtype} tensors on {pool.device} with 16-byte aligned rows")
             if any(ext > 1 and s == 0 for s, ext in zip(st, t.shape)):
                 raise ValueError("out must not be a broadcast view")
-    if b == 0 or num_rows == 0:
-        return out
-    kd, vd = (L.Tensor(*_desc(t, "NHD")) for t in out)
-    with torch.cuda.device(pool.device):
-        L.check(L.lib.sqattn_paged_read(pool._address, C.addressof(kd), C.addressof(vd), b, int(num_rows), block_table.data_ptr(),
-                                        block_table.stride(0), block_table.shape[1], starts.data_ptr(),
-                                        None if ends is None else ends.data_ptr(), _stream()))
+        kd, vd = (L.Tensor(*_desc(t, "NHD")) for t in out)
+    if b and num_rows:
+        _on_device(pool, L.lib.sqattn_paged_read, pool._address, C.addressof(kd), C.addressof(vd), b, num_rows, table, stride, pages, at, until)
     return out
+
+
+def _paged_scratch(pool: PagedPool, a, sizes, query):
+    """A workspace for the call; its size follows from ``sizes`` alone and is asked for once."""
+    need = pool._scratch.get(sizes)
+    if need is None:
+        need = query(C.byref(a))
+        if need:
+            pool._scratch[sizes] = need
+    if need:
+        ws = _paged_empty(pool, (need,), (1,), torch.uint8)   # the caching allocator's blocks are 512-byte aligned
+        a.workspace, a.workspace_bytes = ws.data_ptr(), need
+        return ws
+    return None   # refused: the entry point says why
 
 
 def paged_decode(q, pool: PagedPool, block_table, kv_lens, *, pages=None, max_kv_len: int = 0, sm_scale: float = 0.0,
@@ -577,19 +627,28 @@ def paged_decode(q, pool: PagedPool, block_table, kv_lens, *, pages=None, max_kv
     knows one below the block table's (0: none).  A sequence without keys gets zeros and an LSE of -inf."""
     poll_device_status(pool.device)
     qd, b, hq = _paged_query(pool, q, layout)
-    _paged_index(pool, block_table, b, kv_lens=kv_lens)
-    if pages is not None and (pages.dtype != torch.int32 or pages.dim() != 3 or pages.shape[:2] != (b, pool.num_kv_heads) or
-                              not pages.is_contiguous() or pages.device != pool.device):
-        raise ValueError(f"pages must be a contiguous int32 [{b}, {pool.num_kv_heads}, n] on {pool.device}, got {tuple(pages.shape)} {pages.dtype}")
-    out = torch.empty(q.shape, dtype=out_dtype or pool.dtype, device=q.device)
-    lse = torch.empty(b, hq, 1, dtype=torch.float32, device=q.device) if return_lse else None
+    table, stride, max_pages = _paged_table(pool, block_table, b)
+    lens = _paged_ints(pool, kv_lens, b, "kv_lens")
+    listed = list_at = 0
+    if pages is not None:
+        if pages.dtype is not torch.int32 or pages.dim() != 3 or pages.shape[:2] != (b, pool.num_kv_heads) or \
+                not pages.is_contiguous() or pages.get_device() != pool.device_index:
+            raise ValueError(f"pages must be a contiguous int32 [{b}, {pool.num_kv_heads}, n] on {pool.device}, got {tuple(pages.shape)} {pages.dtype}")
+        listed, list_at = pages.shape[2], pages.data_ptr()
+        if listed == 0 and b:
+            raise ValueError("pages lists no page")
+    d = pool.head_dim
+    out_dtype = out_dtype or pool.dtype
+    out_code = _dt(out_dtype)
+    out = _paged_empty(pool, (b, 1, hq, d) if layout == "NHD" else (b, hq, 1, d), (hq * d, hq * d, d, 1) if layout == "NHD" else (hq * d, d, d, 1), out_dtype)
+    lse = _paged_empty(pool, (b, hq, 1), (hq, 1, 1), torch.float32) if return_lse else None
     if b:
         a = L.PagedDecodeArgs.from_buffer(bytearray(_PAGED_DECODE_ARGS.pack(
-            pool._address, *qd, *_desc(out, layout), 0 if lse is None else lse.data_ptr(), block_table.data_ptr(), block_table.stride(0),
-            kv_lens.data_ptr(), 0 if pages is None else pages.data_ptr(), b, hq, block_table.shape[1],
-            0 if pages is None else pages.shape[2], _dt(out.dtype), int(max_kv_len), float(sm_scale), 0, 0)))
-        with torch.cuda.device(pool.device):
-            _run_decode(a, q.device, L.lib.sqattn_paged_decode_workspace_bytes, L.lib.sqattn_paged_decode)
+            pool._address, *qd, out.data_ptr(), hq * d, d, hq * d, 0 if lse is None else lse.data_ptr(), table, stride, lens, list_at,
+            b, hq, max_pages, listed, out_code, int(max_kv_len), float(sm_scale), 0, 0)))
+        ws = _paged_scratch(pool, a, ("decode", b, hq, max_pages, listed, max_kv_len), L.lib.sqattn_paged_decode_workspace_bytes)
+        _on_device(pool, L.lib.sqattn_paged_decode, C.byref(a))
+        del ws
     return (out, lse) if return_lse else out
 
 
@@ -599,12 +658,16 @@ def paged_select(q, pool: PagedPool, block_table, kv_lens, num_pages: int, *, si
     to, ascending, -1 behind the last: the first ``sink_pages``, the last ``recent_pages`` and those whose key bounds allow the
     highest scores."""
     qd, b, hq = _paged_query(pool, q, layout)
-    _paged_index(pool, block_table, b, kv_lens=kv_lens)
-    out = torch.empty(b, pool.num_kv_heads, int(num_pages), dtype=torch.int32, device=q.device)
+    table, stride, max_pages = _paged_table(pool, block_table, b)
+    lens = _paged_ints(pool, kv_lens, b, "kv_lens")
+    if num_pages <= 0:
+        raise ValueError(f"num_pages {num_pages} must be positive")
+    num_pages = int(num_pages)
+    out = _paged_empty(pool, (b, pool.num_kv_heads, num_pages), (pool.num_kv_heads * num_pages, num_pages, 1), torch.int32)
     if b:
         a = L.PagedSelectArgs.from_buffer(bytearray(_PAGED_SELECT_ARGS.pack(
-            pool._address, *qd, block_table.data_ptr(), block_table.stride(0), kv_lens.data_ptr(), out.data_ptr(), b, hq,
-            block_table.shape[1], int(num_pages), int(sink_pages), int(recent_pages), 0, 0)))
-        with torch.cuda.device(pool.device):
-            _run_decode(a, q.device, L.lib.sqattn_paged_select_workspace_bytes, L.lib.sqattn_paged_select)
+            pool._address, *qd, table, stride, lens, out.data_ptr(), b, hq, max_pages, num_pages, int(sink_pages), int(recent_pages), 0, 0)))
+        ws = _paged_scratch(pool, a, ("select", b, max_pages), L.lib.sqattn_paged_select_workspace_bytes)
+        _on_device(pool, L.lib.sqattn_paged_select, C.byref(a))
+        del ws
     return out

@@ -59,22 +59,39 @@ __device__ __forceinline__ uint32_t max16x2(uint32_t a, uint32_t b) {
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 
+// the same with a NaN in either as the result
+template <bool BF16>
+__device__ __forceinline__ uint32_t min16x2_nan(uint32_t a, uint32_t b) {
+  uint32_t r;
+  if (BF16) asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  else asm("min.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+template <bool BF16>
+__device__ __forceinline__ uint32_t max16x2_nan(uint32_t a, uint32_t b) {
+  uint32_t r;
+  if (BF16) asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  else asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+
 // Quantise one row spread over D / 8 consecutive lanes, 8 channels each; every lane gets the scale.  The codes come out as
 // the integers' low bytes (int8) or nibbles (int4), packed in channel order.
 //
 // The code is the nearest integer to the exact quotient x / s.  The product with an approximate 1/s is off by at most
-// 127 * 2^-20, so its nearest integer is the answer unless it lies that close to a half-integer; there the remainder
-// x - code * s decides, which one fused multiply-add gives exactly (x is a multiple of s's last place whenever code != 0,
-// and the difference is below s in magnitude).  That branch is taken by 0.1 % of the values (x = max/2 is the common one).
+// 127 (2^-22 + 2^-24) < 4e-5 (the reciprocal's error, the product's rounding), so its nearest integer is the answer unless it
+// lies within 1e-4 of a half-integer; there the remainder x - code * s decides, which one fused multiply-add gives exactly (x is
+// a multiple of s's last place whenever code != 0, and the difference is below s in magnitude).  x = max/2 is the common case
+// there.  The kernel is bound by issuing these instructions about as much as by memory, so fp32 goes in pairs.
 template <int FMT, int D, bool BF16>
 __device__ __forceinline__ void quantise_row8(const uint4& x, float& scale, uint32_t (&packed)[2]) {
   constexpr int kLanes = D / 8;
   constexpr uint32_t kNonFinite = BF16 ? 0x7f80u : 0x7c00u;
   constexpr float kRound = 12582912.0f;  // 1.5 * 2^23: added, it leaves the nearest integer in the low bits
-  uint32_t a = __vmaxu2(__vmaxu2(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu), __vmaxu2(x.z & 0x7fff7fffu, x.w & 0x7fff7fffu));
+  uint32_t a = max16x2_nan<BF16>(max16x2_nan<BF16>(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu), max16x2_nan<BF16>(x.z & 0x7fff7fffu, x.w & 0x7fff7fffu));
 #pragma unroll
-  for (int o = kLanes / 2; o > 0; o >>= 1) a = __vmaxu2(a, __shfl_xor_sync(0xffffffffu, a, o));
-  const uint32_t top = max(a & 0xffffu, a >> 16);
+  for (int o = kLanes / 2; o > 0; o >>= 1) a = max16x2_nan<BF16>(a, __shfl_xor_sync(0xffffffffu, a, o));
+  const uint32_t top = max(a & 0x7fffu, (a >> 16) & 0x7fffu);
   const bool finite = top < kNonFinite;
   const float s = fmaxf(to_f32<BF16>(static_cast<uint16_t>(top)) * kv_code_step<FMT>(), kKvSmallestScale);
   scale = finite ? s : __int_as_float(0x7fc00000);
@@ -82,14 +99,19 @@ __device__ __forceinline__ void quantise_row8(const uint4& x, float& scale, uint
   float f[8];
   unpack8<BF16>(x, f);
   uint32_t c[8];
-  bool near_half = false;
+  float off = 0.0f;  // how far from its integer the furthest of the products is
+  const uint64_t inv2 = f32x2_pack(inv, inv), round2 = f32x2_pack(kRound, kRound);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float t = f[i] * inv, r = t + kRound;
-    near_half |= fabsf(t - (r - kRound)) > 0.499f;
-    c[i] = __float_as_uint(r);
+  for (int i = 0; i < 4; ++i) {
+    const uint64_t t = f32x2_mul(f32x2_pack(f[2 * i], f[2 * i + 1]), inv2), r = f32x2_add(t, round2), d = f32x2_sub(t, f32x2_sub(r, round2));
+    float r0, r1, d0, d1;
+    f32x2_unpack(r, r0, r1);
+    f32x2_unpack(d, d0, d1);
+    off = fmaxf(off, fmaxf(fabsf(d0), fabsf(d1)));
+    c[2 * i] = __float_as_uint(r0);
+    c[2 * i + 1] = __float_as_uint(r1);
   }
-  if (near_half) {
+  if (off > 0.4999f) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const float r = __uint_as_float(c[i]) - kRound, e = __fmaf_rn(-r, s, f[i]), half = 0.5f * s;
@@ -124,17 +146,20 @@ struct PagedWriteParams {
   const int* counts;     // [B] or null: number of new rows
 };
 
-// One CTA per (page that new rows fall into, KV head, sequence): it alone writes that page's rows and bounds, so the bounds
-// need no atomics.  D / 8 lanes hold a row, 8 channels each; the rows of the page are dealt to the CTA's lane groups.
+// One CTA per (KV head, page that new rows fall into, sequence): it alone writes that page's rows and bounds, so the bounds
+// need no atomics.  D / 8 lanes hold a row, 8 channels each; the rows of the page are dealt to the CTA's lane groups, whose
+// loads of kWriteRows rows are in flight together.  Heads are the fastest index, so that CTAs that run together read the pieces
+// of the same rows.
+constexpr int kWriteRows = 4;
 template <int FMT, int D, bool BF16>
 __global__ void __launch_bounds__(128) paged_write_kernel(const __grid_constant__ PagedWriteParams p) {
   constexpr int kLanes = D / 8, kGroups = 128 / kLanes;
-  const int b = blockIdx.z, h = blockIdx.y;
+  const int b = blockIdx.z, h = blockIdx.x;
   const int ps = 1 << p.pool.ps_shift;
   const int pos = p.positions[b];
   const int count = p.counts ? min(max(p.counts[b], 0), p.rows) : p.rows;
   if (pos < 0) return;
-  const long long index = (pos >> p.pool.ps_shift) + static_cast<long long>(blockIdx.x);
+  const long long index = (pos >> p.pool.ps_shift) + static_cast<long long>(blockIdx.y);
   const long long first = index * ps - pos;  // new row that falls on the page's row 0 (negative: the page was begun before)
   if (first >= count) return;
   const int page = page_of(p.table, b, index, p.pool.num_pages);
@@ -147,38 +172,48 @@ __global__ void __launch_bounds__(128) paged_write_kernel(const __grid_constant_
   const uint8_t* vb = p.v + 2 * (b * p.v_sb + h * p.v_sh + c * 8);
   constexpr uint32_t kInf = BF16 ? 0x7f807f80u : 0x7c007c00u, kMinusInf = BF16 ? 0xff80ff80u : 0xfc00fc00u;
   uint32_t lo[4] = {kInf, kInf, kInf, kInf}, hi[4] = {kMinusInf, kMinusInf, kMinusInf, kMinusInf};
-  // every lane group runs the same number of steps: the shuffles of a row's scale need whole warps
-  for (int base = r0; base < r1; base += kGroups) {
-    const int r = base + grp;
-    const bool on = r < r1;
-    uint4 kx = make_uint4(0, 0, 0, 0), vx = make_uint4(0, 0, 0, 0);
-    if (on) {
-      kx = *reinterpret_cast<const uint4*>(kb + 2 * (first + r) * p.k_sn);
-      vx = *reinterpret_cast<const uint4*>(vb + 2 * (first + r) * p.v_sn);
-      const uint32_t w[4] = {kx.x, kx.y, kx.z, kx.w};
+  for (int base = r0; base < r1; base += kGroups * kWriteRows) {
+    uint4 kx[kWriteRows], vx[kWriteRows];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) { lo[i] = min16x2<BF16>(lo[i], w[i]); hi[i] = max16x2<BF16>(hi[i], w[i]); }
-    }
-    const long long row = block + r;
-    if (FMT == kKvNative) {
-      if (on) {
-        reinterpret_cast<uint4*>(p.pool.k_pages)[row * kLanes + c] = kx;
-        reinterpret_cast<uint4*>(p.pool.v_pages)[row * kLanes + c] = vx;
+    for (int u = 0; u < kWriteRows; ++u) {
+      const int r = base + u * kGroups + grp;
+      kx[u] = vx[u] = make_uint4(0, 0, 0, 0);
+      if (r < r1) {
+        kx[u] = *reinterpret_cast<const uint4*>(kb + 2 * (first + r) * p.k_sn);
+        vx[u] = *reinterpret_cast<const uint4*>(vb + 2 * (first + r) * p.v_sn);
       }
-    } else {
-      float ks, vs;
-      uint32_t kc[2], vc[2];
-      quantise_row8<FMT, D, BF16>(kx, ks, kc);
-      quantise_row8<FMT, D, BF16>(vx, vs, vc);
+    }
+#pragma unroll
+    for (int u = 0; u < kWriteRows; ++u) {
+      if (base + u * kGroups >= r1) break;   // of the whole CTA: the shuffles of a row's scale need whole warps
+      const int r = base + u * kGroups + grp;
+      const bool on = r < r1;
       if (on) {
-        if (FMT == kKvInt8) {
-          reinterpret_cast<uint2*>(p.pool.k_pages)[row * kLanes + c] = make_uint2(kc[0], kc[1]);
-          reinterpret_cast<uint2*>(p.pool.v_pages)[row * kLanes + c] = make_uint2(vc[0], vc[1]);
-        } else {
-          reinterpret_cast<uint32_t*>(p.pool.k_pages)[row * kLanes + c] = kc[0];
-          reinterpret_cast<uint32_t*>(p.pool.v_pages)[row * kLanes + c] = vc[0];
+        const uint32_t w[4] = {kx[u].x, kx[u].y, kx[u].z, kx[u].w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { lo[i] = min16x2<BF16>(lo[i], w[i]); hi[i] = max16x2<BF16>(hi[i], w[i]); }
+      }
+      const long long row = block + r;
+      if (FMT == kKvNative) {
+        if (on) {
+          reinterpret_cast<uint4*>(p.pool.k_pages)[row * kLanes + c] = kx[u];
+          reinterpret_cast<uint4*>(p.pool.v_pages)[row * kLanes + c] = vx[u];
         }
-        if (c == 0) { p.pool.k_scale[row] = ks; p.pool.v_scale[row] = vs; }
+      } else {
+        float ks, vs;
+        uint32_t kc[2], vc[2];
+        quantise_row8<FMT, D, BF16>(kx[u], ks, kc);
+        quantise_row8<FMT, D, BF16>(vx[u], vs, vc);
+        if (on) {
+          if (FMT == kKvInt8) {
+            reinterpret_cast<uint2*>(p.pool.k_pages)[row * kLanes + c] = make_uint2(kc[0], kc[1]);
+            reinterpret_cast<uint2*>(p.pool.v_pages)[row * kLanes + c] = make_uint2(vc[0], vc[1]);
+          } else {
+            reinterpret_cast<uint32_t*>(p.pool.k_pages)[row * kLanes + c] = kc[0];
+            reinterpret_cast<uint32_t*>(p.pool.v_pages)[row * kLanes + c] = vc[0];
+          }
+          if (c == 0) { p.pool.k_scale[row] = ks; p.pool.v_scale[row] = vs; }
+        }
       }
     }
   }
@@ -199,22 +234,28 @@ __global__ void __launch_bounds__(128) paged_write_kernel(const __grid_constant_
   }
 }
 
-// 8 channels of a row, in fp32: x is what the row's lane loads (16, 8 or 4 bytes)
+// 8 channels of a row as they lie (16, 8 or 4 bytes) and as 16-bit values
+template <int FMT> struct Piece8 { uint4 a; };
+template <> struct Piece8<kKvInt8> { uint2 a; };
+template <> struct Piece8<kKvInt4> { uint32_t a; };
 template <int FMT, bool BF16>
-__device__ __forceinline__ void load_row8(const uint8_t* pages, const float* scales, long long row, int lanes, int c, float (&f)[8]) {
-  if (FMT == kKvNative) {
-    unpack8<BF16>(reinterpret_cast<const uint4*>(pages)[row * lanes + c], f);
+__device__ __forceinline__ uint4 piece8_values(const Piece8<FMT>& x, float scale) {
+  if constexpr (FMT == kKvNative) {
+    return x.a;
   } else {
-    const float s = scales[row];
-    if (FMT == kKvInt8) {
-      const uint2 w = reinterpret_cast<const uint2*>(pages)[row * lanes + c];
+    // a biased code under the exponent of 2^23 is 2^23 + code + bias: two instructions, a conversion of its own runs at a quarter
+    // of the rate
+    float f[8];
+    if constexpr (FMT == kKvInt8) {
+      const uint32_t w[2] = {x.a.x ^ 0x80808080u, x.a.y ^ 0x80808080u};
 #pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = static_cast<float>(static_cast<int8_t>((i < 4 ? w.x : w.y) >> (8 * (i & 3)))) * s;
+      for (int i = 0; i < 8; ++i) f[i] = (__uint_as_float(__byte_perm(w[i >> 2], 0x4b000000u, 0x7650 + (i & 3))) - 8388736.0f) * scale;
     } else {
-      const uint32_t w = reinterpret_cast<const uint32_t*>(pages)[row * lanes + c];
+      const uint32_t w = x.a ^ 0x88888888u;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = static_cast<float>(static_cast<int>(w << (28 - 4 * i)) >> 28) * s;
+      for (int i = 0; i < 8; ++i) f[i] = (__uint_as_float(((w >> (4 * i)) & 15u) | 0x4b000000u) - 8388616.0f) * scale;
     }
+    return pack8<BF16>(f);
   }
 }
 
@@ -223,34 +264,61 @@ struct PagedReadParams {
   BlockTable table;
   uint8_t *k, *v;  // [B, rows, Hkv, D] through element strides
   long long k_sb, k_sh, k_sn, v_sb, v_sh, v_sn;
-  int batch, rows;
+  int rows, rows_per_cta;
   const int* starts;  // [B] position of the first row read
   const int* ends;    // [B] or null: rows at or past this position are zeros
 };
 
-// Row i of sequence b is position starts[b] + i; rows outside the sequence or the table are written as zeros.  One thread
-// takes 8 channels of a row of keys and of values.
+// Row i of sequence b is position starts[b] + i; rows outside the sequence or the table are written as zeros.  A CTA takes up
+// to kReadRows rows of a sequence, a thread 8 channels of a row's keys and values at a time (so that a warp's stores are
+// contiguous), kReadPieces of them in flight.  Where the rows lie is looked up once, by one thread a row.
+constexpr int kReadRows = 32;
+constexpr int kReadPieces = 4;
 template <int FMT, int D, bool BF16>
 __global__ void __launch_bounds__(256) paged_read_kernel(const __grid_constant__ PagedReadParams p) {
-  constexpr int kLanes = D / 8;
-  const long long total = static_cast<long long>(p.batch) * p.rows * p.pool.hkv * kLanes;
-  for (long long idx = blockIdx.x * 256ll + threadIdx.x; idx < total; idx += 256ll * gridDim.x) {
-    const int c = static_cast<int>(idx % kLanes);
-    long long rest = idx / kLanes;
-    const int h = static_cast<int>(rest % p.pool.hkv);
-    rest /= p.pool.hkv;
-    const int i = static_cast<int>(rest % p.rows), b = static_cast<int>(rest / p.rows);
-    const long long pos = static_cast<long long>(p.starts[b]) + i;
+  __shared__ long long at[kReadRows];   // row of the pool for head 0, -1: none
+  const int b = blockIdx.y, i0 = blockIdx.x * p.rows_per_cta, rows = min(p.rows_per_cta, p.rows - i0);
+  if (static_cast<int>(threadIdx.x) < rows) {
+    const long long pos = static_cast<long long>(p.starts[b]) + i0 + threadIdx.x;
     const bool inside = pos >= 0 && (!p.ends || pos < p.ends[b]);
     const int page = inside ? page_of(p.table, b, pos >> p.pool.ps_shift, p.pool.num_pages) : -1;
-    float k[8] = {0, 0, 0, 0, 0, 0, 0, 0}, v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (page >= 0) {
-      const long long row = (((static_cast<long long>(page) * p.pool.hkv + h)) << p.pool.ps_shift) + (pos & ((1 << p.pool.ps_shift) - 1));
-      load_row8<FMT, BF16>(p.pool.k_pages, p.pool.k_scale, row, kLanes, c, k);
-      load_row8<FMT, BF16>(p.pool.v_pages, p.pool.v_scale, row, kLanes, c, v);
+    at[threadIdx.x] = page < 0 ? -1ll : ((static_cast<long long>(page) * p.pool.hkv) << p.pool.ps_shift) + (pos & ((1 << p.pool.ps_shift) - 1));
+  }
+  __syncthreads();
+  constexpr int kParts = D / 8;
+  const int per_row = p.pool.hkv * kParts, total = rows * per_row;
+  uint8_t* ko = p.k + 2 * (b * p.k_sb + i0 * p.k_sn);
+  uint8_t* vo = p.v + 2 * (b * p.v_sb + i0 * p.v_sn);
+  const Piece8<FMT>* kp = reinterpret_cast<const Piece8<FMT>*>(p.pool.k_pages);
+  const Piece8<FMT>* vp = reinterpret_cast<const Piece8<FMT>*>(p.pool.v_pages);
+  for (int j0 = threadIdx.x; j0 < total; j0 += 256 * kReadPieces) {
+    Piece8<FMT> k[kReadPieces], v[kReadPieces];
+    float ks[kReadPieces], vs[kReadPieces];
+    bool there[kReadPieces];
+#pragma unroll
+    for (int u = 0; u < kReadPieces; ++u) {
+      const int j = j0 + u * 256, i = j / per_row, rest = j - i * per_row, h = rest / kParts, c = rest % kParts;
+      const long long first = j < total ? at[i] : -1ll, r = first + (static_cast<long long>(h) << p.pool.ps_shift);
+      there[u] = first >= 0;
+      ks[u] = vs[u] = 1.0f;
+      if (there[u]) {
+        k[u] = kp[r * kParts + c];
+        v[u] = vp[r * kParts + c];
+        if (FMT != kKvNative) { ks[u] = p.pool.k_scale[r]; vs[u] = p.pool.v_scale[r]; }
+      }
     }
-    *reinterpret_cast<uint4*>(p.k + 2 * (b * p.k_sb + h * p.k_sh + i * p.k_sn + c * 8)) = pack8<BF16>(k);
-    *reinterpret_cast<uint4*>(p.v + 2 * (b * p.v_sb + h * p.v_sh + i * p.v_sn + c * 8)) = pack8<BF16>(v);
+#pragma unroll
+    for (int u = 0; u < kReadPieces; ++u) {
+      const int j = j0 + u * 256, i = j / per_row, rest = j - i * per_row, h = rest / kParts, c = rest % kParts;
+      if (j >= total) break;
+      uint4 kx = make_uint4(0, 0, 0, 0), vx = kx;
+      if (there[u]) {
+        kx = piece8_values<FMT, BF16>(k[u], ks[u]);
+        vx = piece8_values<FMT, BF16>(v[u], vs[u]);
+      }
+      *reinterpret_cast<uint4*>(ko + 2 * (i * p.k_sn + h * p.k_sh + c * 8)) = kx;
+      *reinterpret_cast<uint4*>(vo + 2 * (i * p.v_sn + h * p.v_sh + c * 8)) = vx;
+    }
   }
 }
 

@@ -32,21 +32,6 @@ __device__ __forceinline__ int held_pages(const PagedSelectParams& p, int b) {
   return static_cast<int>(min(n, static_cast<long long>(p.table.max_pages)));
 }
 
-template <bool BF16>
-__device__ __forceinline__ uint32_t min16x2_nan(uint32_t a, uint32_t b) {
-  uint32_t r;
-  if (BF16) asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-  else asm("min.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-  return r;
-}
-template <bool BF16>
-__device__ __forceinline__ uint32_t max16x2_nan(uint32_t a, uint32_t b) {
-  uint32_t r;
-  if (BF16) asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-  else asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-  return r;
-}
-
 constexpr int kScorePages = 4;                                   // pages per lane group, loaded ahead of their use
 __host__ __device__ constexpr int score_pages_per_cta(int d) { return 256 / (d / 8) * kScorePages; }
 

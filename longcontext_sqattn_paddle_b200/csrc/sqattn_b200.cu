@@ -1397,7 +1397,8 @@ int sqattn_paged_write(const sqattn_paged_pool* pool, const sqattn_tensor* k, co
   p.v_sb = v->stride_b; p.v_sh = v->stride_h; p.v_sn = v->stride_n;
   p.rows = num_rows; p.positions = positions; p.counts = counts;
   const int64_t touched = (static_cast<int64_t>(num_rows) + pool->page_size - 2) / pool->page_size + 1;  // pages, wherever the rows start
-  const dim3 grid(static_cast<unsigned>(touched), pool->num_kv_heads, batch);
+  if (touched > 65535) return fail(SQATTN_ERR_UNSUPPORTED, "paged write: %d rows fall into more than 65535 pages", num_rows);
+  const dim3 grid(pool->num_kv_heads, static_cast<unsigned>(touched), batch);
 #define SQ_LAUNCH(F, D, B) paged_write_kernel<F, D, B><<<grid, 128, 0, stream>>>(p)
   SQ_PAGED_DISPATCH(pool, SQ_LAUNCH);
 #undef SQ_LAUNCH
@@ -1421,8 +1422,11 @@ int sqattn_paged_read(const sqattn_paged_pool* pool, const sqattn_tensor_out* k,
   p.k = static_cast<uint8_t*>(k->ptr); p.v = static_cast<uint8_t*>(v->ptr);
   p.k_sb = k->stride_b; p.k_sh = k->stride_h; p.k_sn = k->stride_n;
   p.v_sb = v->stride_b; p.v_sh = v->stride_h; p.v_sn = v->stride_n;
-  p.batch = batch; p.rows = num_rows; p.starts = starts; p.ends = ends;
-  const int grid = elementwise_grid(static_cast<long long>(batch) * num_rows * pool->num_kv_heads * (pool->head_dim / 8), 256);
+  p.rows = num_rows; p.starts = starts; p.ends = ends;
+  // rows of a CTA: enough for four pieces a thread, fewer heads more rows
+  const int pieces = pool->num_kv_heads * (pool->head_dim / 8);
+  p.rows_per_cta = std::max(1, std::min(kReadRows, (1024 + pieces - 1) / pieces));
+  const dim3 grid((num_rows + p.rows_per_cta - 1) / p.rows_per_cta, batch);
 #define SQ_LAUNCH(F, D, B) paged_read_kernel<F, D, B><<<grid, 256, 0, stream>>>(p)
   SQ_PAGED_DISPATCH(pool, SQ_LAUNCH);
 #undef SQ_LAUNCH

@@ -107,7 +107,7 @@ __device__ __forceinline__ void quantise_row8(const uint4& x, float& scale, uint
     float r0, r1, d0, d1;
     f32x2_unpack(r, r0, r1);
     f32x2_unpack(d, d0, d1);
-    off = fmaxf(off, fmaxf(fabsf(d0), fabsf(d1)));
+    off = max3(off, fabsf(d0), fabsf(d1));
     c[2 * i] = __float_as_uint(r0);
     c[2 * i + 1] = __float_as_uint(r1);
   }
@@ -120,9 +120,9 @@ __device__ __forceinline__ void quantise_row8(const uint4& x, float& scale, uint
       if (e < -half || (e == -half && odd)) --c[i];
     }
   }
-  if (!finite) {
+  if (__any_sync(0xffffffffu, !finite)) {   // a branch that is hardly ever taken
 #pragma unroll
-    for (int i = 0; i < 8; ++i) c[i] = 0u;
+    for (int i = 0; i < 8; ++i) c[i] = finite ? c[i] : 0u;
   }
   if (FMT == kKvInt8) {
 #pragma unroll
@@ -172,28 +172,31 @@ __global__ void __launch_bounds__(128) paged_write_kernel(const __grid_constant_
   const uint8_t* vb = p.v + 2 * (b * p.v_sb + h * p.v_sh + c * 8);
   constexpr uint32_t kInf = BF16 ? 0x7f807f80u : 0x7c007c00u, kMinusInf = BF16 ? 0xff80ff80u : 0xfc00fc00u;
   uint32_t lo[4] = {kInf, kInf, kInf, kInf}, hi[4] = {kMinusInf, kMinusInf, kMinusInf, kMinusInf};
+  const uint8_t* kat = kb + 2 * (first + r0 + grp) * p.k_sn;
+  const uint8_t* vat = vb + 2 * (first + r0 + grp) * p.v_sn;
+  const long long k_step = 2 * kGroups * p.k_sn, v_step = 2 * kGroups * p.v_sn;
+  long long row = block + r0 + grp;
   for (int base = r0; base < r1; base += kGroups * kWriteRows) {
     uint4 kx[kWriteRows], vx[kWriteRows];
 #pragma unroll
     for (int u = 0; u < kWriteRows; ++u) {
-      const int r = base + u * kGroups + grp;
       kx[u] = vx[u] = make_uint4(0, 0, 0, 0);
-      if (r < r1) {
-        kx[u] = *reinterpret_cast<const uint4*>(kb + 2 * (first + r) * p.k_sn);
-        vx[u] = *reinterpret_cast<const uint4*>(vb + 2 * (first + r) * p.v_sn);
+      if (base + u * kGroups + grp < r1) {
+        kx[u] = *reinterpret_cast<const uint4*>(kat);
+        vx[u] = *reinterpret_cast<const uint4*>(vat);
       }
+      kat += k_step;
+      vat += v_step;
     }
 #pragma unroll
-    for (int u = 0; u < kWriteRows; ++u) {
+    for (int u = 0; u < kWriteRows; ++u, row += kGroups) {
       if (base + u * kGroups >= r1) break;   // of the whole CTA: the shuffles of a row's scale need whole warps
-      const int r = base + u * kGroups + grp;
-      const bool on = r < r1;
+      const bool on = base + u * kGroups + grp < r1;
       if (on) {
         const uint32_t w[4] = {kx[u].x, kx[u].y, kx[u].z, kx[u].w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) { lo[i] = min16x2<BF16>(lo[i], w[i]); hi[i] = max16x2<BF16>(hi[i], w[i]); }
       }
-      const long long row = block + r;
       if (FMT == kKvNative) {
         if (on) {
           reinterpret_cast<uint4*>(p.pool.k_pages)[row * kLanes + c] = kx[u];
@@ -286,38 +289,46 @@ __global__ void __launch_bounds__(256) paged_read_kernel(const __grid_constant__
   }
   __syncthreads();
   constexpr int kParts = D / 8;
-  const int per_row = p.pool.hkv * kParts, total = rows * per_row;
+  const int per_row = p.pool.hkv * kParts;
   uint8_t* ko = p.k + 2 * (b * p.k_sb + i0 * p.k_sn);
   uint8_t* vo = p.v + 2 * (b * p.v_sb + i0 * p.v_sn);
   const Piece8<FMT>* kp = reinterpret_cast<const Piece8<FMT>*>(p.pool.k_pages);
   const Piece8<FMT>* vp = reinterpret_cast<const Piece8<FMT>*>(p.pool.v_pages);
-  for (int j0 = threadIdx.x; j0 < total; j0 += 256 * kReadPieces) {
-    Piece8<FMT> k[kReadPieces], v[kReadPieces];
-    float ks[kReadPieces], vs[kReadPieces];
-    bool there[kReadPieces];
+  // a thread keeps to one piece of a row (or to every 256th) and goes down the rows
+  const int rows_at_once = per_row < 256 ? 256 / per_row : 1, my_row = threadIdx.x / per_row < rows_at_once ? threadIdx.x / per_row : rows;
+  for (int col = per_row < 256 ? threadIdx.x % per_row : threadIdx.x; col < per_row; col += 256) {
+    const int h = col / kParts, c = col % kParts;
+    const long long piece = (static_cast<long long>(h) << p.pool.ps_shift) * kParts + c, scale = static_cast<long long>(h) << p.pool.ps_shift;
+    uint8_t* kd = ko + 2 * (h * p.k_sh + c * 8);
+    uint8_t* vd = vo + 2 * (h * p.v_sh + c * 8);
+    for (int i1 = per_row < 256 ? my_row : 0; i1 < rows; i1 += rows_at_once * kReadPieces) {
+      Piece8<FMT> k[kReadPieces], v[kReadPieces];
+      float ks[kReadPieces], vs[kReadPieces];
+      bool there[kReadPieces];
 #pragma unroll
-    for (int u = 0; u < kReadPieces; ++u) {
-      const int j = j0 + u * 256, i = j / per_row, rest = j - i * per_row, h = rest / kParts, c = rest % kParts;
-      const long long first = j < total ? at[i] : -1ll, r = first + (static_cast<long long>(h) << p.pool.ps_shift);
-      there[u] = first >= 0;
-      ks[u] = vs[u] = 1.0f;
-      if (there[u]) {
-        k[u] = kp[r * kParts + c];
-        v[u] = vp[r * kParts + c];
-        if (FMT != kKvNative) { ks[u] = p.pool.k_scale[r]; vs[u] = p.pool.v_scale[r]; }
+      for (int u = 0; u < kReadPieces; ++u) {
+        const int i = i1 + u * rows_at_once;
+        const long long r = i < rows ? at[i] : -1ll;
+        there[u] = r >= 0;
+        ks[u] = vs[u] = 1.0f;
+        if (there[u]) {
+          k[u] = kp[r * kParts + piece];
+          v[u] = vp[r * kParts + piece];
+          if (FMT != kKvNative) { ks[u] = p.pool.k_scale[r + scale]; vs[u] = p.pool.v_scale[r + scale]; }
+        }
       }
-    }
 #pragma unroll
-    for (int u = 0; u < kReadPieces; ++u) {
-      const int j = j0 + u * 256, i = j / per_row, rest = j - i * per_row, h = rest / kParts, c = rest % kParts;
-      if (j >= total) break;
-      uint4 kx = make_uint4(0, 0, 0, 0), vx = kx;
-      if (there[u]) {
-        kx = piece8_values<FMT, BF16>(k[u], ks[u]);
-        vx = piece8_values<FMT, BF16>(v[u], vs[u]);
+      for (int u = 0; u < kReadPieces; ++u) {
+        const int i = i1 + u * rows_at_once;
+        if (i >= rows) break;
+        uint4 kx = make_uint4(0, 0, 0, 0), vx = kx;
+        if (there[u]) {
+          kx = piece8_values<FMT, BF16>(k[u], ks[u]);
+          vx = piece8_values<FMT, BF16>(v[u], vs[u]);
+        }
+        *reinterpret_cast<uint4*>(kd + 2 * i * p.k_sn) = kx;
+        *reinterpret_cast<uint4*>(vd + 2 * i * p.v_sn) = vx;
       }
-      *reinterpret_cast<uint4*>(ko + 2 * (i * p.k_sn + h * p.k_sh + c * 8)) = kx;
-      *reinterpret_cast<uint4*>(vo + 2 * (i * p.v_sn + h * p.v_sh + c * 8)) = vx;
     }
   }
 }

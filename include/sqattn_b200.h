@@ -417,7 +417,8 @@ typedef struct {
 
 /* Write new rows: row i < counts[b] (counts NULL: i < num_rows) of k, v [B, Hkv, num_rows, D] becomes position
  * positions[b] + i of sequence b (positions, counts: device int32 [B]; a negative position writes nothing for that
- * sequence).  Position 0 of a page starts its bounds anew, later ones extend them.  Two sequences of one call must not
+ * sequence).  Position 0 of a page starts its bounds anew, later ones extend them (a row written again leaves them as wide as
+ * they were).  Two sequences of one call must not
  * write into the same page.  Rows 16-byte aligned. */
 int sqattn_paged_write(const sqattn_paged_pool* pool, const sqattn_tensor* k, const sqattn_tensor* v, int32_t batch,
                        int32_t num_rows, const int32_t* block_table, int64_t table_stride, int32_t max_pages,

@@ -35,35 +35,57 @@ __device__ __forceinline__ int held_pages(const PagedSelectParams& p, int b) {
 constexpr int kScorePages = 4;                                   // pages per lane group, loaded ahead of their use
 __host__ __device__ constexpr int score_pages_per_cta(int d) { return 256 / (d / 8) * kScorePages; }
 
+// Sum of x[j] over the LANES lanes of a group for each of the four j; lane c of the group gets the sum of j = c & 3.  Lanes give
+// away half of their values at a time, so that four sums take 10 shuffles and not 32.
+template <int LANES>
+__device__ __forceinline__ double group_sums4(const double (&x)[4], int c) {
+  const bool odd = c & 1, high = c & 2;
+  double a = odd ? x[1] : x[0], z = odd ? x[3] : x[2];
+  a += __shfl_xor_sync(0xffffffffu, odd ? x[0] : x[1], 1);
+  z += __shfl_xor_sync(0xffffffffu, odd ? x[2] : x[3], 1);
+  double s = high ? z : a;
+  s += __shfl_xor_sync(0xffffffffu, high ? a : z, 2);
+#pragma unroll
+  for (int o = 4; o < LANES; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  return s;
+}
+
 // D / 8 lanes take a page: 8 channels each, of which a 16-byte load brings the minima and another the maxima.  The larger of
-// u min and u max is the product with the bound of u's sign, so a channel costs one DFMA.  Bound by the bounds' bytes: 512 a
-// page and KV head at D = 128.
+// u min and u max is the product with the bound of u's sign, so a channel costs one DFMA.  Bound by the bounds' bytes (512 a
+// page and KV head at D = 128) and the latency of three dependent loads, so a CTA goes over several groups of pages and has
+// the next ones in flight.
 template <int D, bool BF16>
-__global__ void __launch_bounds__(256) paged_score_kernel(const __grid_constant__ PagedSelectParams p) {
-  constexpr int kLanes = D / 8, kPer = score_pages_per_cta(D);
+__global__ void __launch_bounds__(256, 3) paged_score_kernel(const __grid_constant__ PagedSelectParams p) {
+  constexpr int kLanes = D / 8, kGroups = 256 / kLanes, kPer = score_pages_per_cta(D);
   __shared__ double u_s[D];
   griddep_launch();
   const int h = blockIdx.y, b = blockIdx.z;
   const int grp = threadIdx.x / kLanes, c = threadIdx.x % kLanes;
-  const int first = blockIdx.x * kPer + grp;
-  uint4 lo[kScorePages], hi[kScorePages];
+  int first = blockIdx.x * kPer + grp;
   int page[kScorePages];
+  auto look_up = [&](int at) {
 #pragma unroll
-  for (int j = 0; j < kScorePages; ++j) page[j] = page_of(p.table, b, first + j * (256 / kLanes), p.pool.num_pages);   // beside the length
+    for (int j = 0; j < kScorePages; ++j) page[j] = page_of(p.table, b, at + j * kGroups, p.pool.num_pages);
+  };
+  look_up(first);   // beside the length
   const int held = held_pages(p, b);
   if (held <= p.budget || static_cast<int>(blockIdx.x) * kPer >= held) return;   // all of them are taken: nothing to score
+  uint4 lo[kScorePages], hi[kScorePages];
+  unsigned on = 0;   // which of the pages there are
+  auto load = [&](int at) {
+    on = 0;
 #pragma unroll
-  for (int j = 0; j < kScorePages; ++j)
-    if (first + j * (256 / kLanes) >= held) page[j] = -1;
-#pragma unroll
-  for (int j = 0; j < kScorePages; ++j) {
-    lo[j] = hi[j] = make_uint4(0, 0, 0, 0);
-    if (page[j] >= 0) {
-      const uint4* row = reinterpret_cast<const uint4*>(p.pool.k_bounds) + (static_cast<long long>(page[j]) * p.pool.hkv + h) * 2 * kLanes;
-      lo[j] = row[c];
-      hi[j] = row[kLanes + c];
+    for (int j = 0; j < kScorePages; ++j) {
+      lo[j] = hi[j] = make_uint4(0, 0, 0, 0);
+      if (page[j] >= 0 && at + j * kGroups < held) {
+        const uint4* row = reinterpret_cast<const uint4*>(p.pool.k_bounds) + (static_cast<long long>(page[j]) * p.pool.hkv + h) * 2 * kLanes;
+        lo[j] = row[c];
+        hi[j] = row[kLanes + c];
+        on |= 1u << j;
+      }
     }
-  }
+  };
+  load(first);
   if (threadIdx.x < D) {
     double s = 0.0;
 #pragma unroll 8
@@ -78,23 +100,37 @@ __global__ void __launch_bounds__(256) paged_score_kernel(const __grid_constant_
   for (int i = 0; i < 8; ++i) u[i] = u_s[c * 8 + i];
 #pragma unroll
   for (int i = 0; i < 4; ++i) sign[i] = (u[2 * i] >= 0.0 ? 0x0000ffffu : 0u) | (u[2 * i + 1] >= 0.0 ? 0xffff0000u : 0u);
+  unsigned long long* out = p.keys + (static_cast<long long>(b) * p.pool.hkv + h) * p.table.max_pages;
+  const int stride = gridDim.x * kPer;
+  for (int base = blockIdx.x * kPer; base < held; base += stride, first += stride) {
+    const unsigned here = on;
+    uint32_t w[kScorePages][4];   // the bounds that count
 #pragma unroll
-  for (int j = 0; j < kScorePages; ++j) {
-    const uint32_t a[4] = {lo[j].x, lo[j].y, lo[j].z, lo[j].w}, z[4] = {hi[j].x, hi[j].y, hi[j].z, hi[j].w};
-    double s = 0.0;
+    for (int j = 0; j < kScorePages; ++j) {
+      const uint32_t a[4] = {lo[j].x, lo[j].y, lo[j].z, lo[j].w}, z[4] = {hi[j].x, hi[j].y, hi[j].z, hi[j].w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t w = (max16x2_nan<BF16>(a[i], z[i]) & sign[i]) | (min16x2_nan<BF16>(a[i], z[i]) & ~sign[i]);
-      s = fma(u[2 * i], static_cast<double>(to_f32<BF16>(static_cast<uint16_t>(w & 0xffffu))), s);
-      s = fma(u[2 * i + 1], static_cast<double>(to_f32<BF16>(static_cast<uint16_t>(w >> 16))), s);
+      for (int i = 0; i < 4; ++i) w[j][i] = (max16x2_nan<BF16>(a[i], z[i]) & sign[i]) | (min16x2_nan<BF16>(a[i], z[i]) & ~sign[i]);
     }
+    if (base + stride < held) {   // the next group's loads fly while this one is summed
+      look_up(first + stride);
+      load(first + stride);
+    }
+    double s[kScorePages];
 #pragma unroll
-    for (int o = kLanes / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    const int i = first + j * (256 / kLanes);
-    if (c == 0 && i < held) {
-      unsigned long long key = page[j] >= 0 ? ordered_key(s) : 0ull;
+    for (int j = 0; j < kScorePages; ++j) {
+      s[j] = 0.0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        s[j] = fma(u[2 * i], static_cast<double>(to_f32<BF16>(static_cast<uint16_t>(w[j][i] & 0xffffu))), s[j]);
+        s[j] = fma(u[2 * i + 1], static_cast<double>(to_f32<BF16>(static_cast<uint16_t>(w[j][i] >> 16))), s[j]);
+      }
+    }
+    const double mine = group_sums4<kLanes>(s, c);
+    const int i = first + (c & 3) * kGroups;
+    if (c < kScorePages && i < held) {
+      unsigned long long key = (here >> c) & 1u ? ordered_key(mine) : 0ull;
       if (i < p.sink_pages || i >= held - p.recent_pages) key = ~0ull;
-      p.keys[(static_cast<long long>(b) * p.pool.hkv + h) * p.table.max_pages + i] = key;
+      out[i] = key;
     }
   }
 }
@@ -155,7 +191,7 @@ __device__ __forceinline__ int chunk_place(unsigned marked, int j, const int* co
 // again in every round.
 __global__ void __launch_bounds__(1024) paged_pick_kernel(const __grid_constant__ PagedSelectParams p) {
   __shared__ int hist[kPickBins], scratch[32], found[3];
-  __shared__ unsigned long long red[2][32];
+  __shared__ uint32_t red[2][32];
   griddep_launch();
   griddep_wait();  // the keys come from the kernel launched just before, the lengths from anywhere
   const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -183,40 +219,26 @@ __global__ void __launch_bounds__(1024) paged_pick_kernel(const __grid_constant_
   };
   load(0);
   int want = p.budget - p.sink_pages - p.recent_pages;
-  unsigned long long lo = ~0ull, hi = 0ull;
+  // bounds of the keys by their high words
+  uint32_t low_word = ~0u, high_word = 0u;
   for (int i0 = 0; i0 < held; i0 += kPickChunk) {
     if (i0 > 0) load(i0);
 #pragma unroll
     for (int j = 0; j < kPickKeys; ++j)
-      if ((in >> j) & 1u) { lo = min(lo, k[j]); hi = max(hi, k[j]); }
+      if ((in >> j) & 1u) { low_word = min(low_word, static_cast<uint32_t>(k[j] >> 32)); high_word = max(high_word, static_cast<uint32_t>(k[j] >> 32)); }
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    lo = min(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-    hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-  }
-  if (lane == 0) { red[0][warp] = lo; red[1][warp] = hi; }
+  low_word = __reduce_min_sync(0xffffffffu, low_word);
+  high_word = __reduce_max_sync(0xffffffffu, high_word);
+  if (lane == 0) { red[0][warp] = low_word; red[1][warp] = high_word; }
   __syncthreads();
-  lo = red[0][lane];
-  hi = red[1][lane];
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    lo = min(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-    hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-  }
-  // keys above `hi` are taken, keys below `lo` are not, `want` of those between are.  (hi < ~0: no score has that key.)
+  low_word = __reduce_min_sync(0xffffffffu, red[0][lane]);
+  high_word = __reduce_max_sync(0xffffffffu, red[1][lane]);
+  // (hi < ~0: no score has that key)
+  unsigned long long lo = static_cast<unsigned long long>(low_word) << 32, hi = min((static_cast<unsigned long long>(high_word) << 32) | 0xffffffffull, ~1ull);
+  // keys above `hi` are taken, keys below `lo` are not, `want` of those between are
   unsigned long long from = hi + 1ull;  // what is taken without a look at its place
-  while (want > 0) {
-    const unsigned long long span = hi - lo;
-    const int shift = max(0, 53 - __clzll(span));  // (hi - lo) >> shift < 2048
-    hist[tid] = hist[1024 + tid] = 0;
-    __syncthreads();
-    for (int i0 = 0; i0 < held; i0 += kPickChunk) {
-      if (many) load(i0);
-#pragma unroll
-      for (int j = 0; j < kPickKeys; ++j)
-        if (((in >> j) & 1u) && k[j] >= lo && k[j] <= hi) atomicAdd(&hist[static_cast<int>((k[j] - lo) >> shift)], 1);
-    }
+  // one round: the histogram has been counted; narrows lo .. hi to a bin, true when there is nothing left to decide
+  auto narrow = [&](int shift) {
     __syncthreads();
     // from the highest bin down: thread t has bins 2047 - 2 t and 2046 - 2 t
     const int b0 = kPickBins - 1 - 2 * tid, n0 = hist[b0], n1 = hist[b0 - 1];
@@ -237,8 +259,42 @@ __global__ void __launch_bounds__(1024) paged_pick_kernel(const __grid_constant_
     lo = bin_lo;
     hi = bin_hi;
     from = hi + 1ull;
-    if (inside == want) { from = lo; want = 0; break; }  // all of the bin
-    if (lo == hi) break;                                 // one value: the lowest pages of it
+    if (inside == want) { from = lo; want = 0; return true; }  // all of the bin
+    return lo == hi;                                           // one value: the lowest pages of it
+  };
+  bool done = want == 0;
+  if (!done && !many) {
+    // the first rounds on the upper 32 bits of key - lo, which cost a third of the instructions
+    const int shift = max(0, 32 - __clzll(hi - lo));
+    uint32_t top[kPickKeys];
+#pragma unroll
+    for (int j = 0; j < kPickKeys; ++j) top[j] = static_cast<uint32_t>((k[j] - lo) >> shift);
+    uint32_t above = 0;   // the bits that the rounds have settled
+#pragma unroll
+    for (int round = 0; round < 2; ++round) {
+      if (done) break;
+      const int place = round == 0 ? 21 : 10;
+      hist[tid] = hist[1024 + tid] = 0;
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < kPickKeys; ++j)
+        if (((in >> j) & 1u) && (round == 0 || (top[j] >> 21) == above)) atomicAdd(&hist[(top[j] >> place) & 2047], 1);
+      done = narrow(shift + place);
+      above = found[0];
+      __syncthreads();
+    }
+  }
+  while (!done) {
+    const int shift = max(0, 53 - __clzll(hi - lo));  // (hi - lo) >> shift < 2048
+    hist[tid] = hist[1024 + tid] = 0;
+    __syncthreads();
+    for (int i0 = 0; i0 < held; i0 += kPickChunk) {
+      if (many) load(i0);
+#pragma unroll
+      for (int j = 0; j < kPickKeys; ++j)
+        if (((in >> j) & 1u) && k[j] >= lo && k[j] <= hi) atomicAdd(&hist[static_cast<int>((k[j] - lo) >> shift)], 1);
+    }
+    done = narrow(shift);
     __syncthreads();
   }
   __syncthreads();

@@ -21,7 +21,7 @@ import torch
 import torch.nn.functional as F
 
 from .. import ops
-from ..cache_hub import flash_attn_cache
+from ..cache_hub import PagedKVCache, flash_attn_cache
 from ..sqattn import kernels as K
 
 
@@ -125,7 +125,9 @@ class RandomInitDecoder:
 
     def __init__(self, config: DecoderConfig, max_length: int, dtype=torch.bfloat16, device="cuda:0",
                  attention_type: str = "SQAttn", seed: int = 0, seq_shard: Tuple[int, int] = (0, 1),
-                 with_lm_head: bool = True, shard_layout: str = "contiguous"):
+                 with_lm_head: bool = True, shard_layout: str = "contiguous", paged_kv: Optional[dict] = None):
+        """``paged_kv``: keep the KV cache in pages, with these options of ``cache_hub.PagedKVCache`` (kv_format, page_size,
+        select_pages, ...); None: ``flash_attn_cache``."""
         self.config, self.max_length, self.dtype, self.attention_type = config, max_length, dtype, attention_type
         self.device = torch.device(device)
         self.device_map = str(device)
@@ -150,7 +152,8 @@ class RandomInitDecoder:
         self.cos_sin_cache, self.attention_scaling = yarn_cos_sin_cache(
             self.head_dim, self.base, max_length, self.max_position_embeddings, self.yarn_factor, self.device)
         self.layers = [DecoderLayer(i, c, dtype, self.device, attention_type, g) for i in range(self.num_layers)]
-        self.kv_cache: Optional[flash_attn_cache] = None
+        self.paged_kv = paged_kv
+        self.kv_cache = None   # flash_attn_cache or PagedKVCache
 
     # ---- pieces of a layer (model_hub/qwen.py:292-379) -------------------------------------------------
     def word_embedding(self, inputs_id):
@@ -230,10 +233,14 @@ class RandomInitDecoder:
         query_states = q.view(bsz, seq_len, self.num_heads, self.head_dim)
         key_states = k.view(bsz, seq_len, self.num_key_value_heads, self.head_dim)
         value_states = v.view(bsz, seq_len, self.num_key_value_heads, self.head_dim)
-        lens = None if dev is not None else [x + 1 for x in self.kv_cache.valid_length_host]
-        key_states, value_states = self.kv_cache.decode_update_kv_cache(key_states, value_states, layer_idx)
-        attn_out = layer.decode_attention(query_states, key_states, value_states, None, kv_lens=lens,
-                                          kv_lens_device=None if dev is None else dev[1])
+        if self.paged_kv is not None:
+            self.kv_cache.decode_update_kv_cache(key_states, value_states, layer_idx)
+            attn_out = self.kv_cache.decode_attention(query_states, layer_idx)
+        else:
+            lens = None if dev is not None else [x + 1 for x in self.kv_cache.valid_length_host]
+            key_states, value_states = self.kv_cache.decode_update_kv_cache(key_states, value_states, layer_idx)
+            attn_out = layer.decode_attention(query_states, key_states, value_states, None, kv_lens=lens,
+                                              kv_lens_device=None if dev is None else dev[1])
         hidden_states = residual + self.wo(attn_out, layer, bsz, seq_len, dim)
         residual = hidden_states
         normed = self.layernorm(hidden_states, layer.post_attention_layernorm_variance_epsilon,
@@ -277,6 +284,9 @@ class RandomInitDecoder:
         if kc is None or kc.valid_length is None or not kc.allocated:
             raise RuntimeError("capture_decode_step needs a prefilled, GPU-resident cache")
         dev = self.device
+        if self.paged_kv is not None:
+            for b in range(batch_size):   # a replayed step takes no pages of its own
+                kc.reserve(b, kc.max_length)
         self._g_ids = torch.zeros(batch_size, 1, dtype=torch.int64, device=dev)
         self._g_pos = torch.full((1,), kc.context, dtype=torch.int64, device=dev)
         self._g_lens = torch.zeros(batch_size, dtype=torch.int32, device=dev)
@@ -290,6 +300,7 @@ class RandomInitDecoder:
         # warm-up outside capture (library workspaces, lazy initialisation), then put the state back: the rows it
         # wrote at index valid_length are overwritten by the first real step
         host, vl = self._host_state(), kc.valid_length.clone()
+        bounds = kc.bounds() if self.paged_kv is not None else None
         side = torch.cuda.Stream(dev)
         side.wait_stream(torch.cuda.current_stream(dev))
         with torch.cuda.stream(side):
@@ -297,6 +308,8 @@ class RandomInitDecoder:
         torch.cuda.current_stream(dev).wait_stream(side)
         torch.cuda.synchronize(dev)
         kc.valid_length.copy_(vl)
+        if bounds is not None:
+            kc.restore_bounds(bounds)
         self._g_pos.fill_(host[0])
         self._set_host_state(host)
         self._graph = torch.cuda.CUDAGraph()
@@ -315,6 +328,12 @@ class RandomInitDecoder:
 
     # ---- generation (model_hub/LLM.py:160-235, model_hub/qwen.py:269-290) ------------------------------
     def init_kv_cache(self, real_input_length, valid_start):
+        if self.paged_kv is not None:
+            self.kv_cache = PagedKVCache(
+                valid_start=valid_start, layer_num=self.num_layers, batch_size=self.batch_size,
+                max_length=self.max_new_length + real_input_length, num_key_value_heads=self.num_key_value_heads,
+                num_heads=self.num_heads, head_dim=self.head_dim, dtype=self.dtype, device=self.device, **self.paged_kv)
+            return
         self.kv_cache = flash_attn_cache(
             valid_start=valid_start, layer_num=self.num_layers, batch_size=self.batch_size,
             max_length=self.max_new_length + real_input_length, num_key_value_heads=self.num_key_value_heads,

@@ -102,3 +102,23 @@ def test_tensors_that_are_refused():
         ops.PagedPool.allocate(3, 16, 2, 64, kv_format="int2")
     with pytest.raises(RuntimeError):
         ops.PagedPool(pages, pages, scale, scale, dtype=torch.float16)   # all well, but no CUDA tensors
+
+
+def test_page_bookkeeping():
+    from longcontext_sqattn_paddle_b200.cache_hub import PageAllocator
+    a = PageAllocator(num_pages=10, page_size=16, batch_size=3, max_pages=6)
+    assert a.reserve(0, 1) == [0] and a.reserve(0, 16) == [] and a.reserve(0, 17) == [1]
+    assert a.reserve(1, 96) == [2, 3, 4, 5, 6, 7] and a.reserve(2, 0) == []
+    with pytest.raises(ValueError):
+        a.reserve(0, 97)
+    with pytest.raises(RuntimeError):
+        a.reserve(2, 33)
+    assert a.pages[2] == [] and len(a.free) == 2              # a refused reservation takes nothing
+    assert a.release(1) == 6 and a.release(1) == 0
+    assert sorted(a.reserve(2, 90)) == [2, 3, 4, 5, 6, 7] and sorted(a.free + a.pages[0] + a.pages[2]) == list(range(10))
+
+
+def test_selection_budgets_that_are_refused():
+    from longcontext_sqattn_paddle_b200.cache_hub import PagedKVCache
+    with pytest.raises(ValueError):
+        PagedKVCache(0, 1, 1, 64, 2, 4, 64, torch.float16, select_pages=2, sink_pages=1, recent_pages=2, device="cpu")

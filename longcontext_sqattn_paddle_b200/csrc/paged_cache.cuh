@@ -7,6 +7,10 @@
 //   s = max(fl32(max|x| * fl32(1/Q)), 2^-100), Q = 127 or 7,   code = nearest integer to x / s (ties to even),   value = code * s.
 // A row with an infinity or a NaN gets the scale NaN and zero codes, so that it reads back as NaN.  The floor of the scale
 // keeps 1/s finite for rows of (nearly) zeros.
+// The paged kernels are launched with programmatic stream serialisation: they become resident while the kernel before them
+// drains and wait for it before they read or write anything.  A decode step is a row of short kernels (append, score, pick,
+// attend, each 3 to 15 us), and launch latency lies between them otherwise.
+//
 // k_bounds [P, Hkv, 2, D] (optional) holds the channel minima and maxima of the page's keys as they were given.
 #pragma once
 #include "prep.cuh"
@@ -154,6 +158,8 @@ constexpr int kWriteRows = 4;
 template <int FMT, int D, bool BF16>
 __global__ void __launch_bounds__(128) paged_write_kernel(const __grid_constant__ PagedWriteParams p) {
   constexpr int kLanes = D / 8, kGroups = 128 / kLanes;
+  griddep_launch();
+  griddep_wait();
   const int b = blockIdx.z, h = blockIdx.x;
   const int ps = 1 << p.pool.ps_shift;
   const int pos = p.positions[b];
@@ -280,6 +286,8 @@ constexpr int kReadPieces = 4;
 template <int FMT, int D, bool BF16>
 __global__ void __launch_bounds__(256) paged_read_kernel(const __grid_constant__ PagedReadParams p) {
   __shared__ long long at[kReadRows];   // row of the pool for head 0, -1: none
+  griddep_launch();
+  griddep_wait();
   const int b = blockIdx.y, i0 = blockIdx.x * p.rows_per_cta, rows = min(p.rows_per_cta, p.rows - i0);
   if (static_cast<int>(threadIdx.x) < rows) {
     const long long pos = static_cast<long long>(p.starts[b]) + i0 + threadIdx.x;

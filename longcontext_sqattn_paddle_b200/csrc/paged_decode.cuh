@@ -173,6 +173,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
   constexpr bool kNative = FMT == kKvNative;
   constexpr uint32_t kAllValid = MT == 2 ? 0x1010u : 0x10101010u;
   griddep_launch();
+  griddep_wait();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int hkv = p.pool.hkv;
   auto store_o = [&](int b, int hq, int d, float x) {

@@ -59,6 +59,7 @@ __global__ void __launch_bounds__(256, 3) paged_score_kernel(const __grid_consta
   constexpr int kLanes = D / 8, kGroups = 256 / kLanes, kPer = score_pages_per_cta(D);
   __shared__ double u_s[D];
   griddep_launch();
+  griddep_wait();
   const int h = blockIdx.y, b = blockIdx.z;
   const int grp = threadIdx.x / kLanes, c = threadIdx.x % kLanes;
   int first = blockIdx.x * kPer + grp;

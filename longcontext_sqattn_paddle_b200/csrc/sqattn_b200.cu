@@ -37,7 +37,7 @@ double sm_scale_log2(int head_dim, int head_dim_og = 0) {
 // none 4.806 ms, the merge kernels only 4.800 ms, merge and decode kernels 5.245 ms (a decode grid that becomes
 // resident behind the running one slows it down), so of those only the merges do by default.  The operator's preparation
 // and its attention kernel do: 8192 tokens, FP8 P: 310 us a call with, 320 without; 1000 tokens: 46.8 and 48.3.
-// SQATTN_B200_OVERLAP (read once) overrides with a bit mask of kernel classes: 1 = merge kernels, 2 = decode kernel,
+// SQATTN_B200_OVERLAP (read once) overrides with a bit mask of kernel classes: 1 = merge and paged-cache kernels, 2 = decode kernel,
 // 4 = preparation and prefill kernels.
 int overlap_mask() {
   static int mask = -1;
@@ -692,10 +692,19 @@ int launch_paged_decode(const sqattn_paged_decode_args* a, const PagedDecodePlan
   SQ_CUDA(cudaFuncSetAttribute(paged_decode_kernel<FMT, D, BF16, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(pl.grid); cfg.blockDim = dim3(Cfg::kWarps * 32); cfg.dynamicSmemBytes = smem; cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = kPagedCluster; attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr; cfg.numAttrs = pl.clusters ? 1 : 0;
+  cudaLaunchAttribute attr[2];
+  unsigned attrs = 0;
+  if (overlap_mask() & 1) {
+    attr[attrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[attrs++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (pl.clusters) {
+    attr[attrs].id = cudaLaunchAttributeClusterDimension;
+    attr[attrs].val.clusterDim.x = kPagedCluster;
+    attr[attrs].val.clusterDim.y = attr[attrs].val.clusterDim.z = 1;
+    ++attrs;
+  }
+  cfg.attrs = attr; cfg.numAttrs = attrs;
   SQ_CUDA(cudaLaunchKernelEx(&cfg, paged_decode_kernel<FMT, D, BF16, NT>, tk, tv, p));
   if (!pl.clusters) {
     const int by_cut = pl.grid > 1 && (pl.grid - 1) * p.groups < a->num_q_heads * a->batch;
@@ -1399,7 +1408,7 @@ int sqattn_paged_write(const sqattn_paged_pool* pool, const sqattn_tensor* k, co
   const int64_t touched = (static_cast<int64_t>(num_rows) + pool->page_size - 2) / pool->page_size + 1;  // pages, wherever the rows start
   if (touched > 65535) return fail(SQATTN_ERR_UNSUPPORTED, "paged write: %d rows fall into more than 65535 pages", num_rows);
   const dim3 grid(pool->num_kv_heads, static_cast<unsigned>(touched), batch);
-#define SQ_LAUNCH(F, D, B) paged_write_kernel<F, D, B><<<grid, 128, 0, stream>>>(p)
+#define SQ_LAUNCH(F, D, B) SQ_CUDA(launch_overlapped(1, paged_write_kernel<F, D, B>, grid, dim3(128), 0, stream, p))
   SQ_PAGED_DISPATCH(pool, SQ_LAUNCH);
 #undef SQ_LAUNCH
   SQ_CUDA(cudaGetLastError());
@@ -1427,7 +1436,7 @@ int sqattn_paged_read(const sqattn_paged_pool* pool, const sqattn_tensor_out* k,
   const int pieces = pool->num_kv_heads * (pool->head_dim / 8);
   p.rows_per_cta = std::max(1, std::min(kReadRows, (1024 + pieces - 1) / pieces));
   const dim3 grid((num_rows + p.rows_per_cta - 1) / p.rows_per_cta, batch);
-#define SQ_LAUNCH(F, D, B) paged_read_kernel<F, D, B><<<grid, 256, 0, stream>>>(p)
+#define SQ_LAUNCH(F, D, B) SQ_CUDA(launch_overlapped(1, paged_read_kernel<F, D, B>, grid, dim3(256), 0, stream, p))
   SQ_PAGED_DISPATCH(pool, SQ_LAUNCH);
 #undef SQ_LAUNCH
   SQ_CUDA(cudaGetLastError());
@@ -1504,8 +1513,8 @@ int sqattn_paged_select(const sqattn_paged_select_args* a, sqattn_stream_t strea
     const int groups = (a->max_pages + per - 1) / per;
     const int rounds = static_cast<int64_t>(groups) * a->pool->num_kv_heads * a->batch > 148 * 3 ? 2 : 1;
     const dim3 grid((groups + rounds - 1) / rounds, a->pool->num_kv_heads, a->batch);
-    if (a->pool->head_dim == 128) { if (bf16) paged_score_kernel<128, true><<<grid, 256, 0, stream>>>(p); else paged_score_kernel<128, false><<<grid, 256, 0, stream>>>(p); }
-    else { if (bf16) paged_score_kernel<64, true><<<grid, 256, 0, stream>>>(p); else paged_score_kernel<64, false><<<grid, 256, 0, stream>>>(p); }
+    if (a->pool->head_dim == 128) { if (bf16) SQ_CUDA(launch_overlapped(1, paged_score_kernel<128, true>, grid, dim3(256), 0, stream, p)); else SQ_CUDA(launch_overlapped(1, paged_score_kernel<128, false>, grid, dim3(256), 0, stream, p)); }
+    else { if (bf16) SQ_CUDA(launch_overlapped(1, paged_score_kernel<64, true>, grid, dim3(256), 0, stream, p)); else SQ_CUDA(launch_overlapped(1, paged_score_kernel<64, false>, grid, dim3(256), 0, stream, p)); }
     SQ_CUDA(cudaGetLastError());
   }
   SQ_CUDA(launch_overlapped(1, paged_pick_kernel, dim3(a->pool->num_kv_heads, a->batch), dim3(1024), 0, stream, p));

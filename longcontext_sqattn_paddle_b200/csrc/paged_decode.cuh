@@ -21,7 +21,8 @@
 //     q as 16-bit integers, a power of two per head high, in a signed high and an unsigned low byte: sums are exact, and q is
 //     off by at most 2^-15 of the head's largest (bf16 channels down to 1/64 of the largest are exact).
 //   codes, output: codes become f16 exactly by exponent tricks; a value's scale multiplies its weight p in fp32, and the product
-//     is rounded to f16 relative to the largest value scale so far (as a power of two), 2^14 high.
+//     is rounded to f16 relative to the largest value scale so far (as a power of two), 2^14 high.  For bf16 outputs that
+//     rounding (2^-11) vanishes beside theirs (2^-8); for f16 outputs, which have the same, the weight is split as below.
 //   The conversions are what costs: on this part an ALU or f16x2 instruction takes an SM quarter 2 clocks, a f16 product
 //     m16n8k16 8.3, an integer product m16n8k32 8.1, and they hardly overlap.
 //   native: p is split into two 16-bit parts, so that its rounding (2^-16 or 2^-22) vanishes beside the output's.
@@ -51,7 +52,7 @@ struct PagedDecodeParams {
   const int* list;  // [B, Hkv, list_len] pages of the sequence to attend to, or null: all of them
   int list_len;
   int max_len;  // what the table, or the caller's bound, holds
-  int batch, hq, groups, q_bf16, o_bf16;
+  int batch, hq, groups, o_bf16;
   int clusters;      // a cluster of kPagedCluster CTAs for each segment: they join its parts themselves
   int q_align;       // bytes that every head's row is aligned to: 16, 4 or 2
   float scale_log2;  // softmax scale * log2(e)
@@ -171,6 +172,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
   using C = PagedDecodeCfg<FMT, D, NT>;
   constexpr int W = C::kWarps, S = C::kStages, ROW = C::kRow, TILE = C::kTile, MT = TILE / 16, NTHR = W * 32, H = 8 * NT;
   constexpr bool kNative = FMT == kKvNative;
+  constexpr bool kTwoParts = kNative || !BF16;   // weights in two 16-bit parts
   constexpr uint32_t kAllValid = MT == 2 ? 0x1010u : 0x10101010u;
   griddep_launch();
   griddep_wait();
@@ -471,7 +473,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
 #pragma unroll
         for (int i = 0; i < D / 4; ++i) {
           const uint16_t w = static_cast<uint16_t>(i & 1 ? v[i / 2] >> 16 : v[i / 2] & 0xffffu);
-          f[i] = p.q_bf16 ? to_f32<true>(w) : to_f32<false>(w);
+          f[i] = to_f32<BF16>(w);
           top = fmaxf(top, fabsf(f[i]));
           if (f[i] != f[i]) top = INFINITY;
         }
@@ -677,7 +679,13 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
                 pb[nt][mt][hi] = movmatrix_trans(head);
                 pl[nt][mt][hi] = movmatrix_trans(BF16 ? pack_bf16x2(w0 - h0, w1 - h1) : pack_f16x2(w0 - h0, w1 - h1));
               } else {
-                pb[nt][mt][hi] = movmatrix_trans(pack_f16x2(w0 * vs[mt][hi], w1 * vs[mt][hi]));
+                const float a = w0 * vs[mt][hi], z = w1 * vs[mt][hi];
+                const uint32_t head = pack_f16x2(a, z);
+                pb[nt][mt][hi] = movmatrix_trans(head);
+                if (kTwoParts) {
+                  const float h0 = to_f32<false>(static_cast<uint16_t>(head & 0xffffu)), h1 = to_f32<false>(static_cast<uint16_t>(head >> 16));
+                  pl[nt][mt][hi] = movmatrix_trans(pack_f16x2(a - h0, z - h1));
+                }
               }
             }
         }
@@ -725,7 +733,10 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
                   bytes_to_h2(lo, ce, a[0], a[1]);
                   bytes_to_h2(hi, ce, a[2], a[3]);
 #pragma unroll
-                  for (int nt = 0; nt < NT; ++nt) mma_16816<false>(o[nt][2 * u + half], a, pb[nt][mt][0], pb[nt][mt][1]);
+                  for (int nt = 0; nt < NT; ++nt) {
+                    mma_16816<false>(o[nt][2 * u + half], a, pb[nt][mt][0], pb[nt][mt][1]);
+                    if (kTwoParts) mma_16816<false>(o[nt][2 * u + half], a, pl[nt][mt][0], pl[nt][mt][1]);
+                  }
                 } else {
 #pragma unroll
                   for (int q = 0; q < 2; ++q) {
@@ -733,7 +744,10 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
                     nibbles_to_h2(lo >> (8 * q), ce, a[0], a[1]);
                     nibbles_to_h2(hi >> (8 * q), ce, a[2], a[3]);
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) mma_16816<false>(o[nt][4 * u + 2 * half + q], a, pb[nt][mt][0], pb[nt][mt][1]);
+                    for (int nt = 0; nt < NT; ++nt) {
+                      mma_16816<false>(o[nt][4 * u + 2 * half + q], a, pb[nt][mt][0], pb[nt][mt][1]);
+                      if (kTwoParts) mma_16816<false>(o[nt][4 * u + 2 * half + q], a, pl[nt][mt][0], pl[nt][mt][1]);
+                    }
                   }
                 }
               }

@@ -1470,7 +1470,7 @@ int sqattn_paged_decode(const sqattn_paged_decode_args* a, sqattn_stream_t strea
   p.batch = a->batch; p.hq = a->num_q_heads; p.groups = a->num_q_heads / pool->num_kv_heads;
   const uintptr_t q_bits = reinterpret_cast<uintptr_t>(a->q.ptr) | static_cast<uintptr_t>(a->q.stride_b * 2) | static_cast<uintptr_t>(a->q.stride_h * 2);
   p.q_align = q_bits % 16 == 0 ? 16 : q_bits % 4 == 0 ? 4 : 2;
-  p.q_bf16 = pool->dtype == SQATTN_BF16; p.o_bf16 = a->o_dtype == SQATTN_BF16;
+  p.o_bf16 = a->o_dtype == SQATTN_BF16;
   const double scale = a->sm_scale > 0.0f ? static_cast<double>(a->sm_scale) : 1.0 / sqrt(static_cast<double>(pool->head_dim));
   p.scale_log2 = std::max(static_cast<float>(scale * 1.4426950408889634), 1e-30f);   // a factor of 0 would turn masked scores into NaN
   uint8_t* ws = static_cast<uint8_t*>(a->workspace);
@@ -1479,9 +1479,7 @@ int sqattn_paged_decode(const sqattn_paged_decode_args* a, sqattn_stream_t strea
   p.piece_o = reinterpret_cast<float*>(ws + pl.piece_off);
   p.plan = reinterpret_cast<int*>(ws + pl.plan_off);
   p.cut = reinterpret_cast<int*>(ws + pl.cut_off);
-  // codes become f16 whatever the queries' type
-#define SQ_LAUNCH(F, D, B) \
-  return p.groups > 8 ? launch_paged_decode<F, D, (F) == kKvNative && B, 2>(a, pl, p, stream) : launch_paged_decode<F, D, (F) == kKvNative && B, 1>(a, pl, p, stream)
+#define SQ_LAUNCH(F, D, B) return p.groups > 8 ? launch_paged_decode<F, D, B, 2>(a, pl, p, stream) : launch_paged_decode<F, D, B, 1>(a, pl, p, stream)
   SQ_PAGED_DISPATCH(pool, SQ_LAUNCH);
 #undef SQ_LAUNCH
   return SQATTN_OK;

@@ -5,7 +5,7 @@ Layout:
   _lib.py, ops.py     ctypes binding and tensor-level wrappers
   sqattn/             host-side mirror of the reference operator surface
                       (attention_fn adapter, kernel launchers)
-  cache_hub/          kmeans clustering and the KV cache
+  cache_hub/          kmeans clustering and the KV caches (contiguous, host-hybrid, clustered, paged)
   dist.py             sequence-parallel prefill and cross-GPU split-KV decode
 
 Importing the package never falls back to a CPU or PyTorch path: without the

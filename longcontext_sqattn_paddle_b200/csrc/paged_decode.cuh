@@ -173,6 +173,8 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
   constexpr int W = C::kWarps, S = C::kStages, ROW = C::kRow, TILE = C::kTile, MT = TILE / 16, NTHR = W * 32, H = 8 * NT;
   constexpr bool kNative = FMT == kKvNative;
   constexpr bool kTwoParts = kNative || !BF16;   // weights in two 16-bit parts
+  // f16 weights are kept 2^14 high, away from that type's subnormal numbers; bf16 has none to fear, and its values could overflow
+  constexpr float kLift = kNative && BF16 ? 0.0f : 14.0f, kUnlift = kNative && BF16 ? 1.0f : 1.0f / 16384.0f;
   constexpr uint32_t kAllValid = MT == 2 ? 0x1010u : 0x10101010u;
   griddep_launch();
   griddep_wait();
@@ -653,7 +655,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
             }
           }
         }
-        // ---- weights, 2^14 high, and their two 16-bit parts (native) or products with the value scales (codes)
+        // ---- weights and their two 16-bit parts, for codes of their products with the value scales
         uint32_t pb[NT][MT][2], pl[NT][MT][2];
         const float inv = __uint_as_float((254u << 23) - vexp);
         if (!kNative) {
@@ -664,7 +666,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         for (int nt = 0; nt < NT; ++nt) {
           float off[2];
 #pragma unroll
-          for (int c = 0; c < 2; ++c) off[c] = 14.0f - (m[nt][c] == -INFINITY ? 0.0f : m[nt][c] * cs[nt][c]);
+          for (int c = 0; c < 2; ++c) off[c] = kLift - (m[nt][c] == -INFINITY ? 0.0f : m[nt][c] * cs[nt][c]);
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -761,14 +763,14 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
 
     // ---- this warp's result of the segment
     const float nan = __int_as_float(0x7fc00000);
-    const float unit = kNative ? 1.0f : __uint_as_float(vexp);
+    const float unit = (kNative ? 1.0f : __uint_as_float(vexp)) * kUnlift;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
 #pragma unroll
         for (int sh = 4; sh < 32; sh <<= 1) l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], sh);
-        if (!ok) l[nt][c] = nan;
+        l[nt][c] = ok ? l[nt][c] * kUnlift : nan;
         m[nt][c] = m[nt][c] == -INFINITY ? -INFINITY : m[nt][c] * cs[nt][c];  // a NaN sum has no maximum of its own
       }
     // channel of o[nt][i][e]; e & 1 is the column
@@ -795,7 +797,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
             }
             if (p.lse && g == 0)
               p.lse[static_cast<long long>(b) * p.hq + h * p.groups + col] =
-                  l[nt][c] != 0.0f ? log2f(l[nt][c]) - 14.0f + (m[nt][c] == -INFINITY ? 0.0f : m[nt][c]) : -INFINITY;
+                  l[nt][c] != 0.0f ? log2f(l[nt][c]) + (m[nt][c] == -INFINITY ? 0.0f : m[nt][c]) : -INFINITY;
           }
         }
     } else {
@@ -871,7 +873,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     }
     if (on) {
       ml[lane * H + head] = den != 0.0f ? f / den : 0.0f;
-      ml[(2 * W + lane) * H + head] = den != 0.0f ? log2f(den) - 14.0f + (top == -INFINITY ? 0.0f : top) : -INFINITY;
+      ml[(2 * W + lane) * H + head] = den != 0.0f ? log2f(den) + (top == -INFINITY ? 0.0f : top) : -INFINITY;
     }
   }
   __syncthreads();

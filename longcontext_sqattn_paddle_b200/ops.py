@@ -586,6 +586,8 @@ def paged_read(pool: PagedPool, block_table, starts, num_rows: int, ends=None, o
     at = _paged_ints(pool, starts, b, "starts")
     until = None if ends is None else _paged_ints(pool, ends, b, "ends")
     num_rows = int(num_rows)
+    if num_rows < 0:
+        raise ValueError(f"num_rows {num_rows} must not be negative")
     hkv, d = pool.num_kv_heads, pool.head_dim
     if out is None:
         shape, strides = (b, num_rows, hkv, d), (num_rows * hkv * d, hkv * d, d, 1)

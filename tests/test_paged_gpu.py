@@ -321,6 +321,38 @@ def test_decode_hands_on_nan_of_rows_that_count(fmt):
     assert out[0, :2].isnan().all() and out[0, 2:].isfinite().all()
 
 
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("n", [20, 500])
+def test_decode_of_values_near_the_types_range(fmt, n):
+    """bf16 values of up to 2^118, one warp's and several warps' keys: sums of weights times values stay in fp32's range."""
+    dtype, d = torch.bfloat16, 128
+    g = _gen(46)
+    table = torch.arange(8, dtype=torch.int32)[None]
+    ref = _empty(fmt, dtype, 8, 1, 64, d)
+    key, value = torch.randn(1, n, 1, d, generator=g).to(dtype), (torch.rand(1, n, 1, d, generator=g) * 2.0 ** 118).to(dtype)
+    PO.write(ref, fmt, key, value, table, [0], [n])
+    q = torch.randn(1, 8, d, generator=g).to(dtype)
+    pool = _cuda(ref)
+    out, lse = _decode(q, pool, dtype, table, [n])
+    assert out.isfinite().all()
+    _check_attention(q.cuda(), pool, fmt, table, [n], out, lse)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("shift", [1, 2])
+def test_decode_of_queries_at_any_address(fmt, shift):
+    ops = _ops()
+    dtype, d = torch.float16, 64
+    pool = _handle(_cuda(_full(fmt, dtype, 8, 2, 16, d, 47)), dtype)
+    table, lens = torch.arange(8, dtype=torch.int32)[None].cuda(), _i32([100])
+    q = torch.randn(1, 1, 6, d, generator=_gen(48)).to(dtype).cuda()
+    odd = torch.zeros(1, 1, 6, d + shift, dtype=dtype, device="cuda")
+    odd[..., shift:] = q
+    assert torch.equal(ops.paged_decode(odd[..., shift:], pool, table, lens), ops.paged_decode(q, pool, table, lens))
+    pages = ops.paged_select(odd[..., shift:], pool, table, lens, 3)
+    assert torch.equal(pages, ops.paged_select(q, pool, table, lens, 3))
+
+
 def test_decode_layouts_types_bounds_and_table_strides():
     ops = _ops()
     dtype, d, hkv, ps, lens = torch.bfloat16, 128, 2, 32, [100, 257]
@@ -498,6 +530,57 @@ def test_captured_step_follows_the_lengths():
         got = [t.clone() for t in captured]
         for a, b in zip(got, step()):
             assert torch.equal(a, b)
+
+
+def test_batches_at_the_limits():
+    """One head of one short sequence; as many sequences as a call takes, empty ones among them; one more is refused."""
+    ops = _ops()
+    dtype, d = torch.bfloat16, 64
+    host = _full("int4", dtype, 64, 1, 16, d, 141)
+    pool_t = _cuda(host)
+    pool = _handle(pool_t, dtype)
+    b = 1024
+    table = torch.randint(0, 64, (b, 3), generator=_gen(142), dtype=torch.int32)
+    lens = torch.randint(-1, 49, (b,), generator=_gen(143)).tolist()
+    q = torch.randn(b, 2, d, generator=_gen(144)).to(dtype)
+    out, lse = _decode(q, pool_t, dtype, table, lens)
+    _check_attention(q.cuda(), pool_t, "int4", table, lens, out, lse)
+    one, l1 = _decode(q[:1, :1], pool_t, dtype, table[:1], [1])
+    _check_attention(q[:1, :1].cuda(), pool_t, "int4", table[:1], [1], one, l1)
+    with pytest.raises(ValueError, match="1024"):
+        ops.paged_decode(torch.zeros(b + 1, 1, 2, d, dtype=dtype, device="cuda"), pool, torch.zeros(b + 1, 3, dtype=torch.int32, device="cuda"), _i32([1] * (b + 1)))
+    none = ops.paged_decode(torch.zeros(0, 1, 2, d, dtype=dtype, device="cuda"), pool, table[:0].cuda(), _i32([]))
+    assert none.shape == (0, 1, 2, d)
+
+
+def test_wrong_tensors_are_refused():
+    ops = _ops()
+    dtype, d = torch.bfloat16, 64
+    pool = _handle(_cuda(_full("int8", dtype, 4, 2, 16, d, 151)), dtype)
+    table, lens = torch.zeros(2, 2, dtype=torch.int32, device="cuda"), _i32([3, 4])
+    q = torch.zeros(2, 1, 4, d, dtype=dtype, device="cuda")
+    rows = torch.zeros(2, 3, 2, d, dtype=dtype, device="cuda")
+    bad_calls = [
+        lambda: ops.paged_decode(q.half(), pool, table, lens), lambda: ops.paged_decode(q.cpu(), pool, table, lens),
+        lambda: ops.paged_decode(q[..., :32], pool, table, lens), lambda: ops.paged_decode(q.expand(2, 2, 4, d), pool, table, lens),
+        lambda: ops.paged_decode(q, pool, table.long(), lens), lambda: ops.paged_decode(q, pool, table[:1], lens),
+        lambda: ops.paged_decode(q, pool, table.cpu(), lens), lambda: ops.paged_decode(q, pool, table, lens.long()),
+        lambda: ops.paged_decode(q, pool, table, lens[:1]), lambda: ops.paged_decode(q, pool, table.t().contiguous().t(), lens),
+        lambda: ops.paged_decode(q, pool, table, lens, layout="HND"), lambda: ops.paged_decode(q, pool, table, lens, out_dtype=torch.float32),
+        lambda: ops.paged_decode(q, pool, table, lens, pages=torch.zeros(2, 2, 0, dtype=torch.int32, device="cuda")),
+        lambda: ops.paged_decode(q, pool, table, lens, pages=torch.zeros(2, 1, 3, dtype=torch.int32, device="cuda")),
+        lambda: ops.paged_decode(q, pool, table, lens, sm_scale=float("nan")), lambda: ops.paged_decode(q, pool, table, lens, max_kv_len=-1),
+        lambda: ops.paged_decode(q[:, :, :3], pool, table, lens),
+        lambda: ops.paged_select(q, pool, table, lens, 0), lambda: ops.paged_select(q, pool, table, lens, 2, sink_pages=2, recent_pages=1),
+        lambda: ops.paged_write(pool, rows.float(), rows.float(), table, lens), lambda: ops.paged_write(pool, rows, rows[:, :2], table, lens),
+        lambda: ops.paged_write(pool, rows[:, :, :1], rows[:, :, :1], table, lens), lambda: ops.paged_write(pool, rows, rows, table, lens, lens[:1]),
+        lambda: ops.paged_read(pool, table, lens, -1), lambda: ops.paged_read(pool, table, lens, 3, out=(rows, rows.half())),
+        lambda: ops.paged_read(pool, table, lens, 3, out=(rows, rows[:1, :1].expand(2, 3, 2, d))),
+    ]
+    for i, call in enumerate(bad_calls):
+        with pytest.raises(ValueError):
+            call()
+            pytest.fail(f"call {i} was not refused")
 
 
 def test_calls_on_two_streams_do_not_share_scratch():

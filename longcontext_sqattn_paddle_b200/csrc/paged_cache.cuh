@@ -156,7 +156,7 @@ struct PagedWriteParams {
 // of the same rows.
 constexpr int kWriteRows = 4;
 template <int FMT, int D, bool BF16>
-__global__ void __launch_bounds__(128) paged_write_kernel(const __grid_constant__ PagedWriteParams p) {
+__global__ void __launch_bounds__(128, 6) paged_write_kernel(const __grid_constant__ PagedWriteParams p) {
   constexpr int kLanes = D / 8, kGroups = 128 / kLanes;
   griddep_launch();
   griddep_wait();
@@ -168,12 +168,10 @@ __global__ void __launch_bounds__(128) paged_write_kernel(const __grid_constant_
   const long long index = (pos >> p.pool.ps_shift) + static_cast<long long>(blockIdx.y);
   const long long first = index * ps - pos;  // new row that falls on the page's row 0 (negative: the page was begun before)
   if (first >= count) return;
-  const int page = page_of(p.table, b, index, p.pool.num_pages);
-  if (page < 0) return;
+  const int page = page_of(p.table, b, index, p.pool.num_pages);   // looked at after the first rows have been asked for
   const int r0 = first < 0 ? static_cast<int>(-first) : 0;
   const int r1 = static_cast<int>(min(static_cast<long long>(ps), count - first));
   const int c = threadIdx.x % kLanes, grp = threadIdx.x / kLanes;
-  const long long block = (static_cast<long long>(page) * p.pool.hkv + h) * ps;  // first row of the page's block
   const uint8_t* kb = p.k + 2 * (b * p.k_sb + h * p.k_sh + c * 8);
   const uint8_t* vb = p.v + 2 * (b * p.v_sb + h * p.v_sh + c * 8);
   constexpr uint32_t kInf = BF16 ? 0x7f807f80u : 0x7c007c00u, kMinusInf = BF16 ? 0xff80ff80u : 0xfc00fc00u;
@@ -181,9 +179,8 @@ __global__ void __launch_bounds__(128) paged_write_kernel(const __grid_constant_
   const uint8_t* kat = kb + 2 * (first + r0 + grp) * p.k_sn;
   const uint8_t* vat = vb + 2 * (first + r0 + grp) * p.v_sn;
   const long long k_step = 2 * kGroups * p.k_sn, v_step = 2 * kGroups * p.v_sn;
-  long long row = block + r0 + grp;
-  for (int base = r0; base < r1; base += kGroups * kWriteRows) {
-    uint4 kx[kWriteRows], vx[kWriteRows];
+  uint4 kx[kWriteRows], vx[kWriteRows];
+  auto load = [&](int base) {
 #pragma unroll
     for (int u = 0; u < kWriteRows; ++u) {
       kx[u] = vx[u] = make_uint4(0, 0, 0, 0);
@@ -194,6 +191,12 @@ __global__ void __launch_bounds__(128) paged_write_kernel(const __grid_constant_
       kat += k_step;
       vat += v_step;
     }
+  };
+  load(r0);
+  if (page < 0) return;
+  long long row = (static_cast<long long>(page) * p.pool.hkv + h) * ps + r0 + grp;
+  for (int base = r0; base < r1; base += kGroups * kWriteRows) {
+    if (base > r0) load(base);
 #pragma unroll
     for (int u = 0; u < kWriteRows; ++u, row += kGroups) {
       if (base + u * kGroups >= r1) break;   // of the whole CTA: the shuffles of a row's scale need whole warps
@@ -284,16 +287,16 @@ struct PagedReadParams {
 constexpr int kReadRows = 32;
 constexpr int kReadPieces = 4;
 template <int FMT, int D, bool BF16>
-__global__ void __launch_bounds__(256) paged_read_kernel(const __grid_constant__ PagedReadParams p) {
+__global__ void __launch_bounds__(256, 4) paged_read_kernel(const __grid_constant__ PagedReadParams p) {
   __shared__ long long at[kReadRows];   // row of the pool for head 0, -1: none
   griddep_launch();
   griddep_wait();
   const int b = blockIdx.y, i0 = blockIdx.x * p.rows_per_cta, rows = min(p.rows_per_cta, p.rows - i0);
   if (static_cast<int>(threadIdx.x) < rows) {
+    const int end = p.ends ? p.ends[b] : 2147483647;   // beside the start: the page does not wait for it
     const long long pos = static_cast<long long>(p.starts[b]) + i0 + threadIdx.x;
-    const bool inside = pos >= 0 && (!p.ends || pos < p.ends[b]);
-    const int page = inside ? page_of(p.table, b, pos >> p.pool.ps_shift, p.pool.num_pages) : -1;
-    at[threadIdx.x] = page < 0 ? -1ll : ((static_cast<long long>(page) * p.pool.hkv) << p.pool.ps_shift) + (pos & ((1 << p.pool.ps_shift) - 1));
+    const int page = page_of(p.table, b, pos >> p.pool.ps_shift, p.pool.num_pages);
+    at[threadIdx.x] = page < 0 || (p.ends && pos >= end) ? -1ll : ((static_cast<long long>(page) * p.pool.hkv) << p.pool.ps_shift) + (pos & ((1 << p.pool.ps_shift) - 1));
   }
   __syncthreads();
   constexpr int kParts = D / 8;

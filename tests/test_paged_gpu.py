@@ -583,6 +583,48 @@ def test_wrong_tensors_are_refused():
             pytest.fail(f"call {i} was not refused")
 
 
+def test_after_a_wait_that_ran_out_results_are_nan_until_it_is_cleared():
+    """The failure is a wait of the cross-GPU merge for a flag that nothing sets: it gives up after a second.  While its word is set
+    every form of the paged decode (clusters, stretches joined by rows and by cuts) returns NaN; then the old results again."""
+    import ctypes as C
+    from longcontext_sqattn_paddle_b200 import _lib as L
+    ops = _ops()
+    dtype, d = torch.bfloat16, 128
+    forms = []
+    for fmt, b, hkv, lens in (("native", 1, 2, [300]), ("int8", 1, 4, [20000]), ("int4", 40, 8, [700] * 40)):
+        per = (max(lens) + 63) // 64
+        pool = _handle(_cuda(_full(fmt, dtype, per + 3, hkv, 64, d, 161)), dtype)
+        table = torch.arange(per, dtype=torch.int32).expand(b, per).contiguous().cuda()
+        q = torch.randn(b, 1, 4 * hkv, d, generator=_gen(162)).to(dtype).cuda()
+        forms.append((q, pool, table, _i32(lens)))
+    clean = [ops.paged_decode(*f, return_lse=True) for f in forms]
+    dev, rows, world = torch.device("cuda", 0), 8, 2
+    ops.poll_device_status(dev)
+    data = [torch.zeros(L.lib.sqattn_peer_merge_data_bytes(world, rows, d) // 4, dtype=torch.int32, device=dev) for _ in range(world)]
+    flags = [torch.zeros(L.lib.sqattn_peer_merge_flag_bytes(world, rows) // 4, dtype=torch.int32, device=dev) for _ in range(world)]
+    epoch, po, pl = torch.zeros(1, dtype=torch.int32, device=dev), torch.randn(rows, d, device=dev), torch.randn(rows, device=dev)
+    out = torch.zeros(rows, d, dtype=dtype, device=dev)
+    a = L.PeerMergeArgs()
+    for i in range(world):
+        a.peer_data[i], a.peer_flags[i] = data[i].data_ptr(), flags[i].data_ptr()
+    a.rank, a.world, a.rows, a.rows_cap, a.head_dim = 0, world, rows, rows, d
+    a.epoch, a.part_o, a.part_lse, a.out, a.o_dtype = epoch.data_ptr(), po.data_ptr(), pl.data_ptr(), out.data_ptr(), L.BF16
+    L.check(L.lib.sqattn_decode_peer_merge(C.byref(a), torch.cuda.current_stream().cuda_stream))
+    torch.cuda.synchronize()
+    with pytest.raises(L.SqattnError):
+        ops.paged_decode(*forms[0])
+    ops._MIRRORS[0][1].value = 0               # a caller that ignored the mirror and carried on
+    for f in forms:
+        o, l = ops.paged_decode(*f, return_lse=True)
+        assert o.isnan().all() and l.isnan().all()
+    with pytest.raises(L.SqattnError):
+        ops.check_device_status()
+    ops.check_device_status()
+    for f, (o, l) in zip(forms, clean):
+        o2, l2 = ops.paged_decode(*f, return_lse=True)
+        assert torch.equal(o, o2) and torch.equal(l, l2)
+
+
 def test_calls_on_two_streams_do_not_share_scratch():
     ops = _ops()
     dtype, d, hkv, hq, ps, lens = torch.bfloat16, 128, 4, 28, 64, [30000]

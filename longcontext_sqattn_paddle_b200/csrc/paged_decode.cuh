@@ -184,6 +184,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     reinterpret_cast<uint16_t*>(p.o)[b * p.o_sb + hq * p.o_sh + d] = p.o_bf16 ? from_f32<true>(x) : from_f32<false>(x);
   };
   const bool gave_up = device_failed();   // asked for here, answered at the first barrier
+  // aligned by an offset: a pointer that went through an integer would be loaded from with generic instructions
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((0u - smem_u32(smem_raw)) & 1023u);
   const uint32_t sbase = smem_u32(smem);
@@ -194,12 +195,18 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
   const uint32_t bars = sbase + C::kBarOff + warp * S * 8;
   volatile uint32_t* info = reinterpret_cast<volatile uint32_t*>(smem + C::kInfoOff) + warp * S;
 
-  // ---- plan: tiles (of one KV head) before each sequence
+  // ---- plan: tiles (of one KV head) before each sequence.  Many lengths are fetched by all warps, or the scan would wait for
+  // each 32 of them in turn
+  const bool many = p.batch > 64;
+  if (many) {
+    for (int b = tid; b < p.batch; b += NTHR) pre[b] = paged_tiles<TILE>(p, paged_len(p, b));
+    __syncthreads();
+  }
   if (warp == 0) {
     int run = 0;
     for (int b0 = 0; b0 < p.batch; b0 += 32) {
       const int b = b0 + lane;
-      const int mine = b < p.batch ? paged_tiles<TILE>(p, paged_len(p, b)) : 0;
+      const int mine = b >= p.batch ? 0 : many ? pre[b] : paged_tiles<TILE>(p, paged_len(p, b));
       int x = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -239,7 +246,6 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     }
     return;
   }
-  // aligned by an offset: a pointer that went through an integer would be loaded from with generic instructions
   // the host has checked that all tiles of a call fit 31 bits
   const int total = pre[p.batch] * hkv;
   const int per = max((total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x), W);
@@ -287,7 +293,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
   if (p.clusters && tid < H) share[H * D + tid] = -INFINITY;
   if (x0 < x1) {
   // this warp's tiles: xw0, xw0 + step, .. below xw1.  In a CTA whose tiles are all of one segment the warps take turns, so that
-  // together they read neighbouring rows (1M tokens native: 348 us in stretches, 338 in turns)
+  // together they read neighbouring rows (1M tokens native, three tiles in flight: 348 us in stretches, 338 in turns)
   int xw0, xw1, step;
   {
     const int b = seq_of(x0), n = pre[b + 1] - pre[b], first = pre[b] * hkv + (x0 - pre[b] * hkv) / n * n;

@@ -18,8 +18,10 @@
 // bound the kernel (a key takes 0.25 KFLOP a head for 128-512 bytes), so the tcgen05 path, which would need 64 or 128
 // rows of queries, has nothing to give here.
 //   codes, scores: integer products m16n8k32 of the keys' bytes as they lie (4-bit codes as the high halves of bytes: a mask) with
-//     q as 16-bit integers, a power of two per head high, in a signed high and an unsigned low byte: sums are exact, and q is
-//     off by at most 2^-15 of the head's largest (bf16 channels down to 1/64 of the largest are exact).
+//     q as 24-bit integers, a power of two per head high, in a signed high and two unsigned lower bytes: sums are exact, and q is
+//     off by at most 2^-23 of the head's largest, half a step of fp32.  Two bytes (2^-15) are not enough beside a head's large
+//     channels: with one of 64 times the others scores were off by 1e-3.  The third product costs 512K int4 tokens 67.0 -> 71.4 us,
+//     64 ragged int4 sequences 76.4 -> 78.8, int8 0.5 %; leaving it out for heads without large channels gains 0.5 us of that.
 //   codes, output: codes become f16 exactly by exponent tricks; a value's scale multiplies its weight p in fp32, and the product
 //     is rounded to f16 relative to the largest value scale so far (as a power of two), 2^14 high.  For bf16 outputs that
 //     rounding (2^-11) vanishes beside theirs (2^-8); for f16 outputs, which have the same, the weight is split as below.
@@ -89,7 +91,7 @@ struct PagedDecodeCfg {
   static_assert(8 * NT * D * 4 <= kRingWarp, "a warp's last piece takes the place of its ring");
 };
 
-// C[16][8] += A[16][32] B[32][8] in integers: signed bytes by the signed high bytes (kHigh) or the unsigned low bytes of 16-bit numbers
+// C[16][8] += A[16][32] B[32][8] in integers: signed bytes by the signed high bytes (kHigh) or the unsigned lower bytes of 24-bit numbers
 template <bool kHigh>
 __device__ __forceinline__ void mma_16832_int(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   if (kHigh)
@@ -443,7 +445,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     const bool whole = step == 1 && seg_first >= xw0 && seg_last <= xw1;
 
     // ---- query heads as the products' 8 columns
-    uint32_t qb[NT][D / 16][2];  // native: [channels 16 i ..][r]; codes: [32 of the channels i / 2, high or low bytes i % 2][r]
+    uint32_t qb[NT][kNative ? D / 16 : D * 3 / 32][2];  // native: [channels 16 i ..][r]; codes: [32 of the channels i / 3, byte from the top i % 3][r]
     float cs[NT][2];             // score factor of this lane's two columns
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -487,23 +489,25 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         }
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        // a power of two brings the largest to [2^14, 2^15); 4-bit codes arrive 16 times as large
+        // a power of two brings the largest to [2^22, 2^23), sums come back in units of 2^8; 4-bit codes arrive 16 times as large
         const uint32_t e = max(__float_as_uint(top) >> 23, 27u);
-        const float up = __uint_as_float((268u - e) << 23);
+        const float up = __uint_as_float((276u - e) << 23);
         const float down = e == 255u ? __int_as_float(0x7fc00000) : p.scale_log2 * __uint_as_float((e - (FMT == kKvInt4 ? 18u : 14u)) << 23);
 #pragma unroll
         for (int j = 0; j < D / 32; ++j)
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            uint32_t hi = 0, lo = 0;
+            uint32_t hi = 0, mid = 0, lo = 0;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {   // bytes of word 2 j + r, or even and odd nibbles of word j
               const uint32_t v = static_cast<uint32_t>(__float2int_rn(f[FMT == kKvInt8 ? 8 * j + 4 * r + i : 8 * j + 2 * i + r] * up));
-              hi |= ((v >> 8) & 0xffu) << (8 * i);
+              hi |= ((v >> 16) & 0xffu) << (8 * i);
+              mid |= ((v >> 8) & 0xffu) << (8 * i);
               lo |= (v & 0xffu) << (8 * i);
             }
-            qb[nt][2 * j][r] = hi;
-            qb[nt][2 * j + 1][r] = lo;
+            qb[nt][3 * j][r] = hi;
+            qb[nt][3 * j + 1][r] = mid;
+            qb[nt][3 * j + 2][r] = lo;
           }
         cs[nt][0] = __shfl_sync(0xffffffffu, down, 8 * t);
         cs[nt][1] = __shfl_sync(0xffffffffu, down, 8 * t + 4);
@@ -573,7 +577,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
               }
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-              int high[4] = {0, 0, 0, 0}, low[4] = {0, 0, 0, 0};
+              int high[4] = {0, 0, 0, 0}, middle[4] = {0, 0, 0, 0}, low[4] = {0, 0, 0, 0};
 #pragma unroll
               for (int j = 0; j < D / 32; ++j) {
                 uint32_t a[4];
@@ -587,11 +591,13 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
                     a[2 + hi] = w[hi][j] & 0xf0f0f0f0u;
                   }
                 }
-                mma_16832_int<true>(high, a[0], a[1], a[2], a[3], qb[nt][2 * j][0], qb[nt][2 * j][1]);
-                mma_16832_int<false>(low, a[0], a[1], a[2], a[3], qb[nt][2 * j + 1][0], qb[nt][2 * j + 1][1]);
+                mma_16832_int<true>(high, a[0], a[1], a[2], a[3], qb[nt][3 * j][0], qb[nt][3 * j][1]);
+                mma_16832_int<false>(middle, a[0], a[1], a[2], a[3], qb[nt][3 * j + 1][0], qb[nt][3 * j + 1][1]);
+                mma_16832_int<false>(low, a[0], a[1], a[2], a[3], qb[nt][3 * j + 2][0], qb[nt][3 * j + 2][1]);
               }
 #pragma unroll
-              for (int e = 0; e < 4; ++e) s[nt][mt][e] = static_cast<float>(high[e] * 256 + low[e]);
+              for (int e = 0; e < 4; ++e)   // the upper two below 2^30, then rounded as fp32 sums are
+                s[nt][mt][e] = fmaf(static_cast<float>(low[e]), 1.0f / 256.0f, static_cast<float>(high[e] * 256 + middle[e]));
             }
           }
           // scales

@@ -1,0 +1,55 @@
+"""The paged cache away from the middle of its range: queries, values and scores of unlike size, infinities and NaN, outputs of
+another type, the forms that only large calls take; against the definitions in 64 bits."""
+import math
+
+import pytest
+import torch
+
+from oracle import paged_oracle as PO
+from test_paged_gpu import DTYPES, FORMATS, _cuda, _decode, _empty, _full, _gen, _handle, _i32, _ops, _table
+
+pytestmark = pytest.mark.gpu
+
+
+def _bounds(q, pool, fmt, table, lens, out_dtype, pages=None, one_part=False):
+    """(o, lse, tolerance of o, tolerance of lse) from the definition.  Half a step of the output's type; of the weights,
+    their rounding (one part of 11 bits where `one_part`, else two parts, 2^-15 at most) and twice the scores' error, as numerator
+    and denominator both have it; sums of n terms in fp32.  A score is off by D fp32 steps of sum |q k| and by the query's
+    conversion, 2^-23 of its largest channel in every one.  Weights below f16's normal numbers: n 2^-39 max |v|."""
+    d, n = q.shape[-1], max(list(lens) + [1])
+    o, lse, spread, size, vmax = PO.attention(q, pool, fmt, table, lens, pages)
+    score = d * 2.0 ** -23 * size
+    if fmt != "native":
+        largest = max(PO.values(pool, "k", fmt, int(page), h, slice(None)).abs().sum(-1).max().item()
+                      for page in table.unique() if 0 <= page < pool["k_pages"].shape[0] for h in range(pool["k_pages"].shape[1]))
+        score = score + 2.0 ** -23 * q.double().abs().amax(-1) * largest / math.sqrt(d)
+    weight = (2.0 ** -11 if one_part else 2.0 ** -15) + 2 * score + n * 2.0 ** -23
+    tol = torch.finfo(out_dtype).eps / 2 * o.abs() + weight[..., None] * spread + n * 2.0 ** -39 * vmax[..., None] + torch.finfo(out_dtype).tiny
+    return o, lse, tol, (score + n * 2.0 ** -23) * 1.4427 + 2.0 ** -22 * (1 + lse.abs())
+
+
+def _within(got, want, tol):
+    assert ((got.double() - want).abs() <= tol).all(), ((got.double() - want).abs() / tol).max()
+
+
+# ---- queries ---------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("fmt", ["int8", "int4"])
+@pytest.mark.parametrize("ratio", [1, 16, 64, 256])
+@pytest.mark.parametrize("d,n", [(128, 100), (64, 5)])
+def test_decode_of_queries_with_a_large_channel(dtype, fmt, ratio, d, n):
+    """One channel of every query is many times the others, and the keys have little in it: the other channels decide."""
+    ref = _empty(fmt, dtype, 2, 2, 64, d)
+    g = _gen(201)
+    key, value = (torch.randn(1, n, 2, d, generator=g) for _ in range(2))
+    key[..., 7] *= 1e-2 / ratio
+    table = torch.arange(2, dtype=torch.int32)[None]
+    PO.write(ref, fmt, key.to(dtype), value.to(dtype), table, [0], [n])
+    q = torch.randn(1, 16, d, generator=g)
+    q[..., 7] = 3.3 * ratio
+    q = q.to(dtype).cuda()
+    pool = _cuda(ref)
+    out, lse = _decode(q, pool, dtype, table, [n])
+    o, l, tol, tol_l = _bounds(q, pool, fmt, table, [n], dtype, one_part=dtype == torch.bfloat16)
+    _within(lse, l, tol_l)
+    _within(out, o, tol)

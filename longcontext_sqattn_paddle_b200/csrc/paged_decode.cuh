@@ -24,7 +24,8 @@
 //     64 ragged int4 sequences 76.4 -> 78.8, int8 0.5 %; leaving it out for heads without large channels gains 0.5 us of that.
 //   codes, output: codes become f16 exactly by exponent tricks; a value's scale multiplies its weight p in fp32, and the product
 //     is rounded to f16 relative to the largest value scale so far (as a power of two), 2^14 high.  For bf16 outputs that
-//     rounding (2^-11) vanishes beside theirs (2^-8); for f16 outputs, which have the same, the weight is split as below.
+//     rounding (2^-11) vanishes beside theirs (2^-8); for f16 outputs, which have the same, the weight is split as below.  The
+//     output's type decides, whatever the queries' is.
 //   The conversions are what costs: on this part an ALU or f16x2 instruction takes an SM quarter 2 clocks, a f16 product
 //     m16n8k16 8.3, an integer product m16n8k32 8.1, and they hardly overlap.
 //   native: p is split into two 16-bit parts, so that its rounding (2^-16 or 2^-22) vanishes beside the output's.
@@ -55,6 +56,7 @@ struct PagedDecodeParams {
   int list_len;
   int max_len;  // what the table, or the caller's bound, holds
   int batch, hq, groups, o_bf16;
+  int q_bf16;        // codes: type of the queries (native: BF16)
   int clusters;      // a cluster of kPagedCluster CTAs for each segment: they join its parts themselves
   int q_align;       // bytes that every head's row is aligned to: 16, 4 or 2
   float scale_log2;  // softmax scale * log2(e)
@@ -167,6 +169,7 @@ __device__ __forceinline__ int paged_tiles(const PagedDecodeParams& p, int len) 
   return static_cast<int>((static_cast<unsigned>(keys) + TILE - 1) / TILE);
 }
 
+// BF16: type of pages and queries where pages are native, of the outputs where they are codes
 template <int FMT, int D, bool BF16, int NT>
 __global__ void __launch_bounds__(PagedDecodeCfg<FMT, D, NT>::kWarps * 32, 1)
 paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
@@ -483,7 +486,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
 #pragma unroll
         for (int i = 0; i < D / 4; ++i) {
           const uint16_t w = static_cast<uint16_t>(i & 1 ? v[i / 2] >> 16 : v[i / 2] & 0xffffu);
-          f[i] = to_f32<BF16>(w);
+          f[i] = p.q_bf16 ? to_f32<true>(w) : to_f32<false>(w);
           top = fmaxf(top, fabsf(f[i]));
           if (f[i] != f[i]) top = INFINITY;
         }

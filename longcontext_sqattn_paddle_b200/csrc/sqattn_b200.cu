@@ -588,9 +588,10 @@ bool rows16(const void* ptr, int64_t sb, int64_t sh, int64_t sn) {  // 16-byte p
 }
 
 // KERNEL<format, head_dim, bf16> for a pool
-#define SQ_PAGED_DISPATCH(POOL, LAUNCH)                                                            \
+#define SQ_PAGED_DISPATCH(POOL, LAUNCH) SQ_PAGED_DISPATCH_TYPE(POOL, (POOL)->dtype, LAUNCH)
+#define SQ_PAGED_DISPATCH_TYPE(POOL, DTYPE, LAUNCH)                                                \
   do {                                                                                             \
-    const bool bf16_ = (POOL)->dtype == SQATTN_BF16;                                               \
+    const bool bf16_ = (DTYPE) == SQATTN_BF16;                                                     \
     if ((POOL)->head_dim == 128) {                                                                 \
       if ((POOL)->format == SQATTN_KV_NATIVE) { if (bf16_) LAUNCH(kKvNative, 128, true); else LAUNCH(kKvNative, 128, false); } \
       else if ((POOL)->format == SQATTN_KV_INT8) { if (bf16_) LAUNCH(kKvInt8, 128, true); else LAUNCH(kKvInt8, 128, false); } \
@@ -1471,6 +1472,7 @@ int sqattn_paged_decode(const sqattn_paged_decode_args* a, sqattn_stream_t strea
   const uintptr_t q_bits = reinterpret_cast<uintptr_t>(a->q.ptr) | static_cast<uintptr_t>(a->q.stride_b * 2) | static_cast<uintptr_t>(a->q.stride_h * 2);
   p.q_align = q_bits % 16 == 0 ? 16 : q_bits % 4 == 0 ? 4 : 2;
   p.o_bf16 = a->o_dtype == SQATTN_BF16;
+  p.q_bf16 = pool->dtype == SQATTN_BF16;
   const double scale = a->sm_scale > 0.0f ? static_cast<double>(a->sm_scale) : 1.0 / sqrt(static_cast<double>(pool->head_dim));
   p.scale_log2 = std::max(static_cast<float>(scale * 1.4426950408889634), 1e-30f);   // a factor of 0 would turn masked scores into NaN
   uint8_t* ws = static_cast<uint8_t*>(a->workspace);
@@ -1480,7 +1482,7 @@ int sqattn_paged_decode(const sqattn_paged_decode_args* a, sqattn_stream_t strea
   p.plan = reinterpret_cast<int*>(ws + pl.plan_off);
   p.cut = reinterpret_cast<int*>(ws + pl.cut_off);
 #define SQ_LAUNCH(F, D, B) return p.groups > 8 ? launch_paged_decode<F, D, B, 2>(a, pl, p, stream) : launch_paged_decode<F, D, B, 1>(a, pl, p, stream)
-  SQ_PAGED_DISPATCH(pool, SQ_LAUNCH);
+  SQ_PAGED_DISPATCH_TYPE(pool, pool->format == SQATTN_KV_NATIVE ? pool->dtype : a->o_dtype, SQ_LAUNCH);
 #undef SQ_LAUNCH
   return SQATTN_OK;
 }

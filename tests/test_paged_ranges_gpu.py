@@ -53,3 +53,21 @@ def test_decode_of_queries_with_a_large_channel(dtype, fmt, ratio, d, n):
     o, l, tol, tol_l = _bounds(q, pool, fmt, table, [n], dtype, one_part=dtype == torch.bfloat16)
     _within(lse, l, tol_l)
     _within(out, o, tol)
+
+
+# ---- outputs of another type -----------------------------------------------------------------------------------------
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype,out_dtype", [(torch.bfloat16, torch.float16), (torch.float16, torch.bfloat16)])
+@pytest.mark.parametrize("group,lens", [(4, [3, 1, 5]), (12, [700])])
+def test_decode_is_as_exact_as_its_outputs_type(fmt, dtype, out_dtype, group, lens):
+    """(Small queries: the scores' own error stays below the weights'.)"""
+    d, hkv, ps = 128, 2, 32
+    per = (max(lens) + ps - 1) // ps
+    pool = _cuda(_full(fmt, dtype, per * len(lens), hkv, ps, d, 211))
+    table = _table(len(lens), per, per * len(lens), 212)
+    q = (torch.randn(len(lens), hkv * group, d, generator=_gen(213)) / 32).to(dtype).cuda()
+    out, lse = _decode(q, pool, dtype, table, lens, out_dtype=out_dtype)
+    o, l, tol, tol_l = _bounds(q, pool, fmt, table, lens, out_dtype, one_part=fmt != "native" and out_dtype == torch.bfloat16)
+    assert out.dtype == out_dtype
+    _within(lse, l, tol_l)
+    _within(out, o, tol)

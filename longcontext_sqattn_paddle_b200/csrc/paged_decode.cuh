@@ -28,7 +28,9 @@
 //     output's type decides, whatever the queries' is.
 //   The conversions are what costs: on this part an ALU or f16x2 instruction takes an SM quarter 2 clocks, a f16 product
 //     m16n8k16 8.3, an integer product m16n8k32 8.1, and they hardly overlap.
-//   native: p is split into two 16-bit parts, so that its rounding (2^-16 or 2^-22) vanishes beside the output's.
+//   native: p is split into two 16-bit parts, so that its rounding (2^-16 or 2^-22) vanishes beside the output's.  A low part
+//     may be zero or negative, so tiles with infinite values take another way: those enter by a product of their own, with 1
+//     for every weight that is not zero.  Looking for them costs 16 loads and 64 multiplications of zero a lane and tile.
 // Channels and keys may enter a product in any order as long as both operands agree, so codes are taken from shared memory
 // in the order in which they lie (16 bytes a lane); `row_perm` below orders the keys so that those loads do not collide.
 #pragma once
@@ -125,6 +127,14 @@ __device__ __forceinline__ float2 cluster_load2(uint32_t addr) {
 __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t a) {
   uint32_t r;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
+  return r;
+}
+// t + 0 * x for two 16-bit numbers: NaN once x is infinite or NaN
+template <bool BF16>
+__device__ __forceinline__ uint32_t add_zero_times(uint32_t x, uint32_t t) {
+  uint32_t r;
+  if (BF16) asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(x), "r"(0u), "r"(t));
+  else asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(x), "r"(0u), "r"(t));
   return r;
 }
 __device__ __forceinline__ uint32_t h2_add(uint32_t a, uint32_t b) {
@@ -543,6 +553,18 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
           fence_proxy_async();
           __syncwarp();
         }
+        bool infinite = false;   // whether any of the tile's values is (or is NaN)
+        if (kNative) {
+          const uint4* at = reinterpret_cast<const uint4*>(smem + (tile - sbase) + C::kTensor) + lane;
+          uint32_t t0 = 0u, t1 = 0u;
+#pragma unroll
+          for (int i = 0; i < C::kTensor / 512; ++i) {
+            const uint4 x = at[i * 32];
+            t0 = add_zero_times<BF16>(x.y, add_zero_times<BF16>(x.x, t0));
+            t1 = add_zero_times<BF16>(x.w, add_zero_times<BF16>(x.z, t1));
+          }
+          infinite = __any_sync(0xffffffffu, ((t0 | t1) & 0x7fff7fffu) != 0u);
+        }
         // ---- scores
         float s[NT][MT][4];
         float vs[MT][2];  // value scales of this lane's keys
@@ -707,7 +729,47 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
             }
         }
         // ---- values
-        if (kNative) {
+        if (kNative && infinite) {
+          constexpr uint32_t kExp = BF16 ? 0x7f807f80u : 0x7c007c00u;
+          constexpr uint16_t kOne = BF16 ? 0x3f80 : 0x3c00;
+          uint32_t any[NT][MT][2];   // 1 where a weight is not zero
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+              for (int hi = 0; hi < 2; ++hi) {
+                uint32_t two = 0u;
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                  const float off = kLift - (m[nt][c] == -INFINITY ? 0.0f : m[nt][c] * cs[nt][c]);
+                  if (ex2_approx(fmaf(s[nt][mt][2 * hi + c], cs[nt][c], off)) > 0.0f) two |= static_cast<uint32_t>(kOne) << (16 * c);
+                }
+                any[nt][mt][hi] = movmatrix_trans(two);
+              }
+#pragma unroll 1
+          for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) {
+              uint32_t a[4], z[4];
+              ldmatrix_x4_trans(tile + vx[i & 3] + mt * (16 * ROW) + (i >> 2) * 2048, a[0], a[1], a[2], a[3]);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const uint32_t those = __vcmpeq2(a[j] & kExp, kExp);
+                z[j] = a[j] & those;
+                a[j] &= ~those;
+              }
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                mma_16816<BF16>(c, z, mt ? any[nt][MT - 1][0] : any[nt][0][0], mt ? any[nt][MT - 1][1] : any[nt][0][1]);
+                mma_16816<BF16>(o[nt][i], a, mt ? pb[nt][MT - 1][0] : pb[nt][0][0], mt ? pb[nt][MT - 1][1] : pb[nt][0][1]);
+                mma_16816<BF16>(o[nt][i], a, mt ? pl[nt][MT - 1][0] : pl[nt][0][0], mt ? pl[nt][MT - 1][1] : pl[nt][0][1]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[nt][i][e] += c[e];
+              }
+            }
+        } else if (kNative) {
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -907,7 +969,6 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
       if (es < 0) continue;
       if (es != seg) break;
       const float2 f = *reinterpret_cast<const float2*>(ml + e * H + col);
-      if (f.x == 0.0f && f.y == 0.0f) continue;   // nothing of the piece was stored, perhaps
       const float4 x = reinterpret_cast<const float4*>((e & 1) ? reinterpret_cast<const float*>(smem + (e >> 1) * C::kRingWarp)
                                                                : p.piece_o + (static_cast<long long>(blockIdx.x) * W + (e >> 1)) * (H * D))[at];
       acc.x += f.x * x.x; acc.y += f.y * x.y; acc.z += f.x * x.z; acc.w += f.y * x.w;
@@ -965,8 +1026,8 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         for (int r = 0; r < kPagedCluster; ++r) {
           // a part without keys has an LSE of -inf and whatever the memory held
           const float f0 = lse[r].x == -INFINITY ? 0.0f : ex2_approx(lse[r].x - top.x), f1 = lse[r].y == -INFINITY ? 0.0f : ex2_approx(lse[r].y - top.y);
-          if (f0 != 0.0f) { acc.x += f0 * x[r].x; acc.z += f0 * x[r].z; }
-          if (f1 != 0.0f) { acc.y += f1 * x[r].y; acc.w += f1 * x[r].w; }
+          if (lse[r].x != -INFINITY) { acc.x += f0 * x[r].x; acc.z += f0 * x[r].z; }
+          if (lse[r].y != -INFINITY) { acc.y += f1 * x[r].y; acc.w += f1 * x[r].w; }
           den.x += f0;
           den.y += f1;
         }

@@ -71,3 +71,39 @@ def test_decode_is_as_exact_as_its_outputs_type(fmt, dtype, out_dtype, group, le
     assert out.dtype == out_dtype
     _within(lse, l, tol_l)
     _within(out, o, tol)
+
+
+# ---- infinities ------------------------------------------------------------------------------------------------------
+# (KV heads, lengths): clusters of CTAs; whole segments of one warp; segments cut between CTAs, joined by cuts and by rows
+FORMS = [(2, [100, 33, 1, 700]), (8, [20, 700, 9, 64] * 10), (1, [30000]), (4, [9000, 20, 8193])]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hkv,lens", FORMS)
+def test_infinite_values_of_keys_that_count(dtype, hkv, lens):
+    """An infinite value makes its channel infinite, however small the key's weight and whatever the parts it is split into;
+    two of unlike sign, or a NaN, make it NaN; every other channel is as without them."""
+    d, ps, group = 128, 64, 3
+    per = (max(lens) + ps - 1) // ps
+    pages = per * len(lens)
+    clean = _full("native", dtype, pages, hkv, ps, d, 221)
+    table = _table(len(lens), per, pages, 222)
+    q = (torch.randn(len(lens), hkv * group, d, generator=_gen(223)) * 6).to(dtype).cuda()
+    host = {n: None if t is None else t.clone() for n, t in clean.items()}
+    inf = float("inf")
+    for i, n in enumerate(lens):
+        for c, (key, x) in enumerate([(0, inf), (n - 1, -inf), (n // 2, float("nan")), (n // 3, inf), (n // 4, -inf), (n // 3, inf)]):
+            page, row = int(table[i, key // ps]), key % ps
+            host["v_pages"][page, :, row, 5 + c % 5], clean["v_pages"][page, :, row, 5 + c % 5] = x, 0.0
+    for i, n in enumerate(lens):   # and one channel with both signs
+        for key, x in ((0, inf), (n - 1, -inf if n > 1 else inf)):
+            host["v_pages"][int(table[i, key // ps]), :, key % ps, 90], clean["v_pages"][int(table[i, key // ps]), :, key % ps, 90] = x, 0.0
+    pool, dev = _cuda(host), table.cuda()
+    out, lse = _decode(q, pool, dtype, table, lens)
+    want = PO.attention(q, pool, "native", dev, lens)[0]
+    o, l, tol, tol_l = _bounds(q, _cuda(clean), "native", dev, lens, dtype)
+    odd = ~want.isfinite()
+    assert odd.any(-1).all() and not odd.all(-1).any()
+    assert torch.equal(out.isnan(), want.isnan()) and torch.equal(out.isinf(), want.isinf()) and torch.equal(out[odd] > 0, want[odd] > 0)
+    _within(out[~odd], o[~odd], tol[~odd])
+    _within(lse, l, tol_l)

@@ -448,8 +448,9 @@ typedef struct {
 
 /* o = softmax(sm_scale * q k^T) v over the first kv_lens[b] cached tokens (or those of them in the listed pages); at most
  * 16 query heads per KV head and 1024 sequences.  Softmax statistics and sums in fp32.  Codes enter the products exactly; with
- * them a query channel is off by at most 2^-23 of its head's largest.  An infinite value of a key whose weight fp32 can hold makes
- * its channel infinite (NaN beside one of the other sign). */
+ * them a query channel is off by at most 2^-23 of its head's largest.  Infinities and NaN go where the formula takes them: an
+ * infinite value of a key whose weight fp32 can hold makes its channel infinite (NaN beside one of the other sign), and a
+ * sequence whose scores are all -inf, or of which one is +inf or NaN, gets NaN (its LSE is -inf or NaN). */
 size_t sqattn_paged_decode_workspace_bytes(const sqattn_paged_decode_args* args);
 int sqattn_paged_decode(const sqattn_paged_decode_args* args, sqattn_stream_t stream);
 

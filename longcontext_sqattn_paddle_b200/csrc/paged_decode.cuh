@@ -31,6 +31,8 @@
 //   native: p is split into two 16-bit parts, so that its rounding (2^-16 or 2^-22) vanishes beside the output's.  A low part
 //     may be zero or negative, so tiles with infinite values take another way: those enter by a product of their own, with 1
 //     for every weight that is not zero.  Looking for them costs 16 loads and 64 multiplications of zero a lane and tile.
+// Scores of -inf (a key with an infinity) count as keys: where all of a sequence's are, the output is NaN as the softmax is, and
+// the LSE -inf.  Until the last join such a part has the LSE kAllMinusInf, one without keys -inf.
 // Channels and keys may enter a product in any order as long as both operands agree, so codes are taken from shared memory
 // in the order in which they lie (16 bytes a lane); `row_perm` below orders the keys so that those loads do not collide.
 #pragma once
@@ -42,6 +44,7 @@
 namespace sq {
 
 constexpr int kPagedMaxBatch = 1024;
+constexpr float kAllMinusInf = -3.402823466e38f;   // below every LSE that a sequence can have
 constexpr int kPagedCluster = 8;
 constexpr int kPagedMaxClusters = 16;  // two to a GPC
 
@@ -128,6 +131,10 @@ __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t a) {
   uint32_t r;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
   return r;
+}
+// what kAllMinusInf stands for in the end
+__device__ __forceinline__ void settle_minus_inf(float& val, float& lse) {
+  if (lse == kAllMinusInf) { val = __int_as_float(0x7fc00000); lse = -INFINITY; }
 }
 // t + 0 * x for two 16-bit numbers: NaN once x is infinite or NaN
 template <bool BF16>
@@ -535,6 +542,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
       for (int i = 0; i < D / 16; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.0f;
     }
     uint32_t vexp = 27u << 23;  // exponent of the largest value scale so far
+    bool keys = false;          // whether there has been any key
 
     for (; xc < seg_end; xc += step) {
       ok = ok && mbar_wait_warp(bars + 8 * st, parity, cta_abort, 401);
@@ -542,6 +550,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
       const uint32_t nv = info[st];
       const uint32_t tile = ring + st * (2 * C::kTensor);
       if (nv != 0) {
+        keys = true;
         if (kNative && nv != kAllValid) {
           // rows behind the sequence (or of a page that is not there) may hold anything: zeros, so that 0 * x is 0
           for (int i = lane; i < TILE * (ROW / 16); i += 32) {
@@ -848,7 +857,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
 #pragma unroll
         for (int sh = 4; sh < 32; sh <<= 1) l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], sh);
         l[nt][c] = ok ? l[nt][c] * kUnlift : nan;
-        m[nt][c] = m[nt][c] == -INFINITY ? -INFINITY : m[nt][c] * cs[nt][c];  // a NaN sum has no maximum of its own
+        m[nt][c] = m[nt][c] != -INFINITY ? m[nt][c] * cs[nt][c] : keys && l[nt][c] == 0.0f ? kAllMinusInf : -INFINITY;  // a NaN sum has no maximum of its own
       }
     // channel of o[nt][i][e]; e & 1 is the column
     auto channel = [&](int i, int e) { return kNative ? 16 * i + g + 8 * (e >> 1) : (D / 8) * g + 2 * i + (e >> 1); };
@@ -859,7 +868,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         for (int c = 0; c < 2; ++c) {
           const int col = nt * 8 + 2 * t + c;
           if (col < p.groups) {
-            const float f = l[nt][c] != 0.0f ? unit / l[nt][c] : 0.0f;
+            const float f = l[nt][c] != 0.0f ? unit / l[nt][c] : keys ? nan : 0.0f;
             uint16_t* row = reinterpret_cast<uint16_t*>(p.o) + b * p.o_sb + static_cast<long long>(h * p.groups + col) * p.o_sh;
 #pragma unroll
             for (int i = 0; i < D / 16; ++i) {
@@ -950,7 +959,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     }
     if (on) {
       ml[lane * H + head] = den != 0.0f ? f / den : 0.0f;
-      ml[(2 * W + lane) * H + head] = den != 0.0f ? log2f(den) + (top == -INFINITY ? 0.0f : top) : -INFINITY;
+      ml[(2 * W + lane) * H + head] = den != 0.0f ? log2f(den) + (top == -INFINITY ? 0.0f : top) : top;
     }
   }
   __syncthreads();
@@ -986,9 +995,11 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       if (col + c >= p.groups) break;
-      const float a0 = c ? acc.y : acc.x, a1 = c ? acc.w : acc.z, l1 = c ? lse.y : lse.x;
+      float a0 = c ? acc.y : acc.x, a1 = c ? acc.w : acc.z, l1 = c ? lse.y : lse.x;
       const int hq = h * p.groups + col + c;
       if (inside) {
+        if (l1 == kAllMinusInf) a1 = __int_as_float(0x7fc00000);
+        settle_minus_inf(a0, l1);
         store_o(sb, hq, d0, a0);
         store_o(sb, hq, d1, a1);
         if (at % (D / 16 * 32) < 4 && p.lse) p.lse[static_cast<long long>(sb) * p.hq + hq] = l1;
@@ -1035,12 +1046,13 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           if (col + c >= p.groups) break;
-          const float sum = c ? den.y : den.x, inv = sum != 0.0f ? 1.0f / sum : 0.0f;
+          const float sum = c ? den.y : den.x;
+          float inv = sum != 0.0f ? 1.0f / sum : 0.0f, l1 = sum != 0.0f ? log2f(sum) + (c ? top.y : top.x) : -INFINITY;
+          settle_minus_inf(inv, l1);
           const int hq = h * p.groups + col + c;
           store_o(sb, hq, d0, (c ? acc.y : acc.x) * inv);
           store_o(sb, hq, d1, (c ? acc.w : acc.z) * inv);
-          if (at % (D / 16 * 32) < 4 && p.lse)
-            p.lse[static_cast<long long>(sb) * p.hq + hq] = sum != 0.0f ? log2f(sum) + (c ? top.y : top.x) : -INFINITY;
+          if (at % (D / 16 * 32) < 4 && p.lse) p.lse[static_cast<long long>(sb) * p.hq + hq] = l1;
         }
       }
   }
@@ -1084,6 +1096,7 @@ __global__ void __launch_bounds__(128 * kMergeGroups) paged_merge_kernel(const _
     if (c0 == c1) return;
     const long long base = (static_cast<long long>(c0) + b * p.pool.hkv + h) * p.groups + head;
     merge_row_partials(p.part_o, p.part_lse, base, p.groups, c1 - c0 + 1, D, sm, val, lse);
+    settle_minus_inf(val, lse);
   }
   if (threadIdx.x < D) {
     reinterpret_cast<uint16_t*>(p.o)[b * p.o_sb + hq * p.o_sh + threadIdx.x] = p.o_bf16 ? from_f32<true>(val) : from_f32<false>(val);

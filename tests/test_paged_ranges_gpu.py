@@ -107,3 +107,43 @@ def test_infinite_values_of_keys_that_count(dtype, hkv, lens):
     assert torch.equal(out.isnan(), want.isnan()) and torch.equal(out.isinf(), want.isinf()) and torch.equal(out[odd] > 0, want[odd] > 0)
     _within(out[~odd], o[~odd], tol[~odd])
     _within(lse, l, tol_l)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hkv,lens", FORMS)
+@pytest.mark.parametrize("first", [0, 1])
+def test_scores_of_minus_infinity(dtype, hkv, lens, first):
+    """Keys whose score is -inf have no weight beside others; where no other is left the softmax is NaN and the LSE -inf, unlike
+    that of a sequence without keys."""
+    d, ps, group = 64, 64, 3
+    lens = lens + [0]
+    per = (max(lens) + ps - 1) // ps
+    pages = per * len(lens)
+    host = _full("native", dtype, pages, hkv, ps, d, 231)
+    table = _table(len(lens), per, pages, 232)
+    q = torch.randn(len(lens), hkv * group, d, generator=_gen(233)).to(dtype)
+    q[..., 3] = q[..., 3].abs() + 1
+    host["k_pages"][..., 3] = -float("inf")            # of every key, but of every second sequence the last three are spared
+    spared = list(range(first, len(lens) - 1, 2))
+    for b in spared:
+        for key in range(max(0, lens[b] - 3), lens[b]):
+            host["k_pages"][int(table[b, key // ps]), :, key % ps, 3] = 0.5
+    out, lse = _decode(q.cuda(), _cuda(host), dtype, table, lens)
+    for b, n in enumerate(lens):
+        if b in spared:
+            assert out[b].isfinite().all() and lse[b].isfinite().all()
+        else:
+            assert (lse[b] == -float("inf")).all() and (out[b].isnan().all() if n else (out[b] == 0).all())
+    if not spared:
+        return
+    few = {n: None if t is None else torch.zeros_like(t) for n, t in host.items()}   # the spared keys by themselves
+    short = torch.arange(len(lens), dtype=torch.int32)[:, None]
+    for b in spared:
+        for i, key in enumerate(range(max(0, lens[b] - 3), lens[b])):
+            for t in ("k_pages", "v_pages"):
+                few[t][b, :, i] = host[t][int(table[b, key // ps]), :, key % ps]
+    rows = torch.tensor(spared)
+    counts = [min(3, lens[b]) for b in spared]
+    o, l, tol, tol_l = _bounds(q[rows].cuda(), _cuda(few), "native", short[rows].cuda(), counts, dtype)
+    _within(out[rows.cuda()], o, tol)
+    _within(lse[rows.cuda()], l, tol_l)

@@ -399,7 +399,8 @@ enum {
 /* One layer's pages, all contiguous: k_pages, v_pages [num_pages, num_kv_heads, page_size, row], a row being head_dim
  * 16-bit values, head_dim int8 codes or head_dim / 2 bytes; k_scale, v_scale [num_pages, num_kv_heads, page_size]
  * (NULL for native pages); k_bounds [num_pages, num_kv_heads, 2, head_dim] 16-bit, the channel minima and maxima of every
- * page's keys as they were given (NULL: not kept, sqattn_paged_select is refused).  page_size 16, 32, 64 or 128.
+ * page's keys as they were given, NaN in a channel where one of them is (NULL: not kept, sqattn_paged_select is refused).
+ * page_size 16, 32, 64 or 128.
  * Codes are symmetric: s = max(fl32(max|x| * fl32(1/Q)), 2^-100), Q = 127 or 7; code = nearest integer to x / s, ties to even;
  * a row that holds an infinity or a NaN gets the scale NaN and reads back as NaN.
  *
@@ -456,7 +457,8 @@ int sqattn_paged_decode(const sqattn_paged_decode_args* args, sqattn_stream_t st
 
 /* Choose pages for sparse attention: per sequence and KV head the first sink_pages and last recent_pages pages it holds
  * and, of the others, those with the highest sum_d max(u_d min_d, u_d max_d), u = the sum of the group's query heads, in
- * fp64 (ties to the lowest page), budget in all.  out (device int32 [B, Hkv, budget]): ascending, -1 behind the last.
+ * fp64 (ties to the lowest page, a sum that is NaN behind all others), budget in all.  out (device int32 [B, Hkv, budget]):
+ * ascending, -1 behind the last.
  * budget >= sink_pages + recent_pages; max_pages <= 131072. */
 typedef struct {
   const sqattn_paged_pool* pool;

@@ -44,26 +44,7 @@ __device__ __forceinline__ int page_of(const BlockTable& t, int b, long long ind
   return (id >= 0 && id < num_pages) ? id : -1;
 }
 
-template <bool BF16>
-__device__ __forceinline__ uint32_t min16x2(uint32_t a, uint32_t b) {
-  if (BF16) {
-    const __nv_bfloat162 r = __hmin2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
-    return *reinterpret_cast<const uint32_t*>(&r);
-  }
-  const __half2 r = __hmin2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
-  return *reinterpret_cast<const uint32_t*>(&r);
-}
-template <bool BF16>
-__device__ __forceinline__ uint32_t max16x2(uint32_t a, uint32_t b) {
-  if (BF16) {
-    const __nv_bfloat162 r = __hmax2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
-    return *reinterpret_cast<const uint32_t*>(&r);
-  }
-  const __half2 r = __hmax2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
-  return *reinterpret_cast<const uint32_t*>(&r);
-}
-
-// the same with a NaN in either as the result
+// the smaller and the larger of two pairs, NaN where either is NaN
 template <bool BF16>
 __device__ __forceinline__ uint32_t min16x2_nan(uint32_t a, uint32_t b) {
   uint32_t r;
@@ -204,7 +185,7 @@ __global__ void __launch_bounds__(128, 6) paged_write_kernel(const __grid_consta
       if (on) {
         const uint32_t w[4] = {kx[u].x, kx[u].y, kx[u].z, kx[u].w};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) { lo[i] = min16x2<BF16>(lo[i], w[i]); hi[i] = max16x2<BF16>(hi[i], w[i]); }
+        for (int i = 0; i < 4; ++i) { lo[i] = min16x2_nan<BF16>(lo[i], w[i]); hi[i] = max16x2_nan<BF16>(hi[i], w[i]); }
       }
       if (FMT == kKvNative) {
         if (on) {
@@ -238,10 +219,10 @@ __global__ void __launch_bounds__(128, 6) paged_write_kernel(const __grid_consta
     const int which = threadIdx.x / (D / 2), ch = threadIdx.x % (D / 2);
     uint32_t x = red[0][which][ch];
 #pragma unroll
-    for (int g = 1; g < kGroups; ++g) x = which ? max16x2<BF16>(x, red[g][which][ch]) : min16x2<BF16>(x, red[g][which][ch]);
+    for (int g = 1; g < kGroups; ++g) x = which ? max16x2_nan<BF16>(x, red[g][which][ch]) : min16x2_nan<BF16>(x, red[g][which][ch]);
     uint32_t* out = reinterpret_cast<uint32_t*>(p.pool.k_bounds) +
                     ((static_cast<long long>(page) * p.pool.hkv + h) * 2 + which) * (D / 2) + ch;
-    if (r0 > 0) x = which ? max16x2<BF16>(x, *out) : min16x2<BF16>(x, *out);
+    if (r0 > 0) x = which ? max16x2_nan<BF16>(x, *out) : min16x2_nan<BF16>(x, *out);
     *out = x;
   }
 }

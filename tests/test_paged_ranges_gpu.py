@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from oracle import paged_oracle as PO
-from test_paged_gpu import DTYPES, FORMATS, _cuda, _decode, _empty, _full, _gen, _handle, _i32, _ops, _table
+from test_paged_gpu import DTYPES, FORMATS, _cuda, _decode, _empty, _full, _gen, _handle, _i32, _ops, _same, _table
 
 pytestmark = pytest.mark.gpu
 
@@ -147,3 +147,29 @@ def test_scores_of_minus_infinity(dtype, hkv, lens, first):
     o, l, tol, tol_l = _bounds(q[rows].cuda(), _cuda(few), "native", short[rows].cuda(), counts, dtype)
     _within(out[rows.cuda()], o, tol)
     _within(lse[rows.cuda()], l, tol_l)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_bounds_of_keys_that_are_nan(dtype, fmt):
+    """NaN in one key, in every key of a page, in rows appended to a page begun before: the channel's bounds are NaN and the page
+    is chosen last."""
+    ops = _ops()
+    d, ps, n = 64, 16, 16 * 12
+    key = torch.randn(1, n, 1, d, generator=_gen(241)).to(dtype)
+    key[0, 3 * ps + 5, 0, 9] = float("nan")
+    key[0, 5 * ps:6 * ps, 0, 11] = float("nan")
+    key[0, 8 * ps + 4, 0, 2] = float("nan")            # the page's first four rows come before
+    key[0, 10 * ps + 1, 0, 30] = float("inf")
+    value = torch.randn(1, n, 1, d, generator=_gen(242)).to(dtype)
+    ref = _empty(fmt, dtype, 12, 1, ps, d)
+    got = _cuda(ref)
+    pool, table = _handle(got, dtype), torch.arange(12, dtype=torch.int32)[None]
+    cut = 8 * ps + 4
+    for a, b in ((0, cut), (cut, n)):
+        ops.paged_write(pool, key[:, a:b].cuda(), value[:, a:b].cuda(), table.cuda(), _i32([a]))
+        PO.write(ref, fmt, key[:, a:b], value[:, a:b], table, [a], [b - a])
+    assert _same(got["k_bounds"], ref["k_bounds"]) and ref["k_bounds"].isnan().any(-1).any(-1).sum() == 3
+    q = torch.randn(1, 1, 2, d, generator=_gen(243)).to(dtype).cuda()
+    most = ops.paged_select(q, pool, table.cuda(), _i32([n]), 9, sink_pages=0, recent_pages=0)
+    assert most[0, 0].tolist() == [i for i in range(12) if i not in (3, 5, 8)]

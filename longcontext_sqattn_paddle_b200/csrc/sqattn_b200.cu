@@ -690,7 +690,9 @@ int launch_paged_decode(const sqattn_paged_decode_args* a, const PagedDecodePlan
   if ((rc = make_tmap_pages(&tk, a->pool->k_pages, a->pool, Cfg::kRow, box_rows, "k_pages"))) return rc;
   if ((rc = make_tmap_pages(&tv, a->pool->v_pages, a->pool, Cfg::kRow, box_rows, "v_pages"))) return rc;
   const int smem = Cfg::total(a->batch, pl.clusters);
-  SQ_CUDA(cudaFuncSetAttribute(paged_decode_kernel<FMT, D, BF16, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  // the limit is the process's and calls run side by side: every call sets it to the same, whatever it takes itself
+  constexpr int kLimit = std::max(Cfg::total(kPagedMaxBatch, false), Cfg::total(kPagedMaxClusters, true));
+  SQ_CUDA(cudaFuncSetAttribute(paged_decode_kernel<FMT, D, BF16, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kLimit));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(pl.grid); cfg.blockDim = dim3(Cfg::kWarps * 32); cfg.dynamicSmemBytes = smem; cfg.stream = stream;
   cudaLaunchAttribute attr[2];

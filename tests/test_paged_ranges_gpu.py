@@ -173,3 +173,47 @@ def test_bounds_of_keys_that_are_nan(dtype, fmt):
     q = torch.randn(1, 1, 2, d, generator=_gen(243)).to(dtype).cuda()
     most = ops.paged_select(q, pool, table.cuda(), _i32([n]), 9, sink_pages=0, recent_pages=0)
     assert most[0, 0].tolist() == [i for i in range(12) if i not in (3, 5, 8)]
+
+
+# ---- calls side by side ----------------------------------------------------------------------------------------------
+def test_calls_of_several_threads_with_unlike_batches():
+    """The calls of one kernel need unlike amounts of shared memory; each gets its own, whatever other threads call meanwhile.
+    (Through the C ABI, which runs without the interpreter's lock.)"""
+    import ctypes as C
+    import threading
+    from longcontext_sqattn_paddle_b200 import _lib as L
+    ops = _ops()
+    dtype, d, n = torch.bfloat16, 64, 4
+    pool = _handle(_cuda(_full("int8", dtype, 8, 1, 16, d, 251)), dtype)
+    calls, kept, want = [], [], []
+    for b in [1024] + [20] * (n - 1):
+        q = torch.randn(b, 1, 4, d, generator=_gen(252)).to(dtype).cuda()
+        table, lens = torch.arange(8, dtype=torch.int32).expand(b, 8).contiguous().cuda(), _i32([1] * b)
+        out = torch.empty_like(q)
+        a = L.PagedDecodeArgs(pool=pool._address, q=L.Tensor(q.data_ptr(), 4 * d, d, 4 * d), o=L.Tensor(out.data_ptr(), 4 * d, d, 4 * d),
+                              block_table=table.data_ptr(), table_stride=8, kv_lens=lens.data_ptr(), batch=b, num_q_heads=4, max_pages=8,
+                              o_dtype=L.BF16)
+        ws = torch.empty(L.lib.sqattn_paged_decode_workspace_bytes(C.byref(a)), dtype=torch.uint8, device="cuda")
+        a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+        calls.append(a)
+        kept.append((q, table, lens, out, ws, torch.cuda.Stream()))
+        want.append(ops.paged_decode(q, pool, table, lens))
+    refused = set()
+
+    def run(i):
+        stream = kept[i][5].cuda_stream
+        torch.zeros(1, device="cuda")
+        for _ in range(4000):
+            if L.lib.sqattn_paged_decode(C.byref(calls[i]), stream):
+                refused.add(L.lib.sqattn_last_error_string())
+
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(n)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not refused
+    for k, w in zip(kept, want):
+        assert torch.equal(k[3], w)

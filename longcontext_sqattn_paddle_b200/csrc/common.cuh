@@ -43,6 +43,21 @@ inline EncodeTiledFn encode_tiled_fn() {
   return fn;
 }
 
+// 4-D map of `ptr` with the 128-byte swizzle.  A host thread that has called nothing of the CUDA runtime yet has no context, which
+// this call of the driver needs: it gets the one of its device.
+inline CUresult encode_tiled_4d(EncodeTiledFn fn, CUtensorMap* out, CUtensorMapDataType type, const void* ptr, const cuuint64_t (&dims)[4],
+                                const cuuint64_t (&strides)[3], const cuuint32_t (&box)[4]) {
+  const cuuint32_t estr[4] = {1, 1, 1, 1};
+  auto encode = [&] {
+    return fn(out, type, 4, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult r = encode();
+  int device = 0;
+  if (r == CUDA_ERROR_INVALID_CONTEXT && cudaGetDevice(&device) == cudaSuccess && cudaSetDevice(device) == cudaSuccess) r = encode();
+  return r;
+}
+
 // 4-D map over a [B, H, N, D] 16-bit tensor given by element strides; box = 64 elements (128 bytes,
 // 128-byte swizzle) x box_rows sequence positions.  Rows past `n` read as zero.
 inline int make_tmap_bhnd(CUtensorMap* out, const void* ptr, int dtype, int64_t sb, int64_t sh, int64_t sn, int b,
@@ -60,10 +75,8 @@ inline int make_tmap_bhnd(CUtensorMap* out, const void* ptr, int dtype, int64_t 
   cuuint64_t strides[3] = {static_cast<cuuint64_t>(sn) * 2, static_cast<cuuint64_t>(sh) * 2,
                            static_cast<cuuint64_t>(sb) * 2};
   cuuint32_t box[4] = {64, static_cast<cuuint32_t>(box_rows), 1, 1};
-  cuuint32_t estr[4] = {1, 1, 1, 1};
-  CUresult r = fn(out, dtype == SQATTN_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
-                  const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  const CUresult r = encode_tiled_4d(fn, out, dtype == SQATTN_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, ptr,
+                                     dims, strides, box);
   if (r != CUDA_SUCCESS) return fail(SQATTN_ERR_CUDA, "%s: cuTensorMapEncodeTiled failed (%d)", name, static_cast<int>(r));
   return SQATTN_OK;
 }

@@ -674,9 +674,7 @@ int make_tmap_pages(CUtensorMap* out, const void* ptr, const sqattn_paged_pool* 
   cuuint64_t dims[4] = {128, block / 128 / halves, static_cast<cuuint64_t>(halves), static_cast<cuuint64_t>(pool->num_pages) * pool->num_kv_heads};
   cuuint64_t strides[3] = {static_cast<cuuint64_t>(128 * halves), 128, block};
   cuuint32_t box[4] = {128, static_cast<cuuint32_t>(box_rows * row_bytes / 128 / halves), static_cast<cuuint32_t>(halves), 1};
-  cuuint32_t estr[4] = {1, 1, 1, 1};
-  CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  const CUresult r = encode_tiled_4d(fn, out, CU_TENSOR_MAP_DATA_TYPE_UINT8, ptr, dims, strides, box);
   if (r != CUDA_SUCCESS) return fail(SQATTN_ERR_CUDA, "%s: cuTensorMapEncodeTiled failed (%d)", name, static_cast<int>(r));
   return SQATTN_OK;
 }

@@ -217,3 +217,26 @@ def test_calls_of_several_threads_with_unlike_batches():
     assert not refused
     for k, w in zip(kept, want):
         assert torch.equal(k[3], w)
+
+
+def test_the_first_call_of_a_host_thread():
+    """A thread that has called nothing of CUDA before."""
+    import ctypes as C
+    import threading
+    from longcontext_sqattn_paddle_b200 import _lib as L
+    ops = _ops()
+    dtype, d = torch.bfloat16, 64
+    pool = _handle(_cuda(_full("int8", dtype, 8, 1, 16, d, 261)), dtype)
+    q = torch.randn(1, 1, 4, d, generator=_gen(262)).to(dtype).cuda()
+    table, lens, out = torch.arange(8, dtype=torch.int32)[None].cuda(), _i32([100]), torch.zeros_like(q)
+    a = L.PagedDecodeArgs(pool=pool._address, q=L.Tensor(q.data_ptr(), 4 * d, d, 4 * d), o=L.Tensor(out.data_ptr(), 4 * d, d, 4 * d),
+                          block_table=table.data_ptr(), table_stride=8, kv_lens=lens.data_ptr(), batch=1, num_q_heads=4, max_pages=8, o_dtype=L.BF16)
+    ws = torch.empty(L.lib.sqattn_paged_decode_workspace_bytes(C.byref(a)), dtype=torch.uint8, device="cuda")
+    a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+    stream, said = torch.cuda.current_stream().cuda_stream, []
+    thread = threading.Thread(target=lambda: said.append((L.lib.sqattn_paged_decode(C.byref(a), stream), L.lib.sqattn_last_error_string())))
+    torch.cuda.synchronize()
+    thread.start()
+    thread.join()
+    assert said[0][0] == L.OK, said
+    assert torch.equal(out, ops.paged_decode(q, pool, table, lens))

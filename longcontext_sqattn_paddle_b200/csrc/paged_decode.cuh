@@ -47,7 +47,7 @@ namespace sq {
 constexpr int kPagedMaxBatch = 1024;
 constexpr float kAllMinusInf = -3.402823466e38f;   // below every LSE that a sequence can have
 constexpr int kPagedCluster = 8;
-constexpr int kPagedMaxClusters = 16;  // two to a GPC
+constexpr int kPagedMaxClusters = 16;  // two to a GPC, and as many as the device has places for
 
 struct PagedDecodeParams {
   PagedPool pool;

@@ -5,6 +5,7 @@
 #include <string.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "common.cuh"
 #include "decode.cuh"
@@ -629,6 +630,34 @@ void paged_decode_shape(int* tile, int* warps) {
   *tile = PagedDecodeCfg<FMT, D, NT>::kTile;
   *warps = PagedDecodeCfg<FMT, D, NT>::kWarps;
 }
+// Clusters of the paged decode that the current device runs at once: its CTAs take an SM each, in every variant, so one variant
+// answers for all.  0 where there is no device.
+int paged_cluster_places() {
+  static std::atomic<int> known[64];   // by device, one more than the answer
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess) { cudaGetLastError(); return 0; }
+  const bool keep = device < 64;
+  if (keep && known[device] > 0) return known[device] - 1;
+  using Cfg = PagedDecodeCfg<kKvNative, 128, 1>;
+  constexpr int kSmem = std::max(Cfg::total(kPagedMaxBatch, false), Cfg::total(kPagedMaxClusters, true));
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = kPagedCluster;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.gridDim = dim3(kPagedMaxClusters * kPagedCluster); cfg.blockDim = dim3(Cfg::kWarps * 32); cfg.dynamicSmemBytes = kSmem;
+  cfg.attrs = attr; cfg.numAttrs = 1;
+  int n = 0;
+  auto* kernel = paged_decode_kernel<kKvNative, 128, true, 1>;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess ||
+      cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) {
+    cudaGetLastError();
+    return 0;
+  }
+  if (keep) known[device] = n + 1;
+  return n;
+}
+
 int plan_paged_decode(const sqattn_paged_decode_args* a, PagedDecodePlan* pl) {
   int rc;
   if ((rc = paged_decode_check(a))) return rc;
@@ -647,19 +676,31 @@ int plan_paged_decode(const sqattn_paged_decode_args* a, PagedDecodePlan* pl) {
     return fail(SQATTN_ERR_UNSUPPORTED, "paged decode: %d sequences of up to %lld keys and %d KV heads are more than a call takes (max_kv_len bounds the keys)",
                 a->batch, static_cast<long long>(keys), pool->num_kv_heads);
   pl->grid = static_cast<int>(std::min<int64_t>(148, (tiles * a->batch + warps - 1) / warps));   // one CTA per SM, a tile for every warp
-  // Few short sequences: a cluster of CTAs for each segment, which joins its parts itself, in one launch.  At 28/4 heads, on the
-  // GPU, with clusters and with stretches and a merge: 1000 keys native 9.5 and 11.8 us, int8 9.5 and 12.6, int4 10.4 and 15.9;
-  // 4000 keys 12.0 and 13.1, 11.7 and 13.4, 11.6 and 16.0; 8000 keys 15.7 and 15.1, 14.3 and 15.0, 13.9 and 16.2.
+  // Few short sequences: a cluster of CTAs for each segment, which joins its parts itself, in one launch, as long as all clusters
+  // find a place at once (15 here; a sixteenth waits for the others: 2000 keys of 16 segments 19 us for 15).  A cluster reads a
+  // segment with 8 SMs, the other form with all of them, so for one segment or a few there is a length where that pays for
+  // its second launch.  On the GPU, clusters and stretches with a merge (us):
+  //   keys           1000          2000          4000          6000          8000
+  //   native, 1     8.4  11.7     9.4  11.6    11.4  12.3    13.8  12.5    15.8  12.3     (segments)
+  //   native, 4     8.6  12.4     9.6  12.9    11.9  13.6    14.1  14.2    16.0  15.2
+  //   native, 15                 10.7  14.0                                18.2  22.0
+  //   int8, 1       8.9  12.4     9.9  12.5    11.1  12.8    12.5  13.1    13.9  12.7
+  //   int8, 4       9.1  13.3    10.0  13.7    11.3  13.2    12.7  13.8    14.1  14.8
+  //   int8, 15                   10.2  13.9                                15.2  20.1
+  //   int4, 1       9.9  15.6    10.1  15.9    11.0  16.0    12.6  15.6    13.6  15.9
+  //   int4, 15                   10.5  15.9                                15.2  19.3
   const int64_t segments = static_cast<int64_t>(a->batch) * pool->num_kv_heads;
-  pl->clusters = segments <= kPagedMaxClusters && keys <= 8192;
-  if (pl->clusters) pl->grid = static_cast<int>(segments) * kPagedCluster;
+  const int64_t longest = pool->format == SQATTN_KV_NATIVE && segments <= 4 ? 4608 : pool->format == SQATTN_KV_INT8 && segments == 1 ? 6656 : 8192;
+  pl->clusters = keys <= longest && segments <= std::min(kPagedMaxClusters, paged_cluster_places());
   const size_t row = static_cast<size_t>(groups) * pool->head_dim * 4;
-  const size_t parts = static_cast<size_t>(pl->grid) + static_cast<size_t>(a->batch) * pool->num_kv_heads;
+  const int widest = std::max(pl->grid, kPagedMaxClusters * kPagedCluster);   // the scratch does not depend on the form
+  if (pl->clusters) pl->grid = static_cast<int>(segments) * kPagedCluster;
+  const size_t parts = static_cast<size_t>(widest) + static_cast<size_t>(a->batch) * pool->num_kv_heads;
   pl->lse_off = align_up(parts * row, 256);
   pl->piece_off = pl->lse_off + align_up(parts * groups * 4, 256);
-  pl->plan_off = pl->piece_off + align_up(static_cast<size_t>(pl->grid) * warps * (groups > 8 ? 16 : 8) * pool->head_dim * 4, 256);
+  pl->plan_off = pl->piece_off + align_up(static_cast<size_t>(widest) * warps * (groups > 8 ? 16 : 8) * pool->head_dim * 4, 256);
   pl->cut_off = pl->plan_off + align_up((static_cast<size_t>(a->batch) + 2) * 4, 256);
-  pl->total = pl->cut_off + align_up(static_cast<size_t>(pl->grid) * 4, 256);
+  pl->total = pl->cut_off + align_up(static_cast<size_t>(widest) * 4, 256);
   return SQATTN_OK;
 }
 

@@ -240,3 +240,22 @@ def test_the_first_call_of_a_host_thread():
     thread.join()
     assert said[0][0] == L.OK, said
     assert torch.equal(out, ops.paged_decode(q, pool, table, lens))
+
+
+# ---- forms of the decode ---------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("b,hkv", [(1, 14), (5, 3), (2, 8), (1, 17)])
+@pytest.mark.parametrize("n", [100, 4609, 6657, 8193])
+def test_decode_on_either_side_of_the_lines_between_its_forms(fmt, b, hkv, n):
+    """As many segments as there are places for clusters, one more; lengths at which the form changes; bounds of the lengths too."""
+    dtype, d, ps = torch.bfloat16, 128, 128
+    per = (n + ps - 1) // ps
+    pool = _cuda(_full(fmt, dtype, per + 2, hkv, ps, d, 271))
+    table = torch.stack([torch.randperm(per + 2, generator=_gen(272 + i))[:per] for i in range(b)]).to(torch.int32).cuda()
+    q = torch.randn(b, hkv, d, generator=_gen(273)).to(dtype).cuda()
+    lens = [n - 7 * i for i in range(b)]
+    o, l, tol, tol_l = _bounds(q, pool, fmt, table, lens, dtype, one_part=True)
+    for bound in (0, n):
+        out, lse = _decode(q, pool, dtype, table, lens, max_kv_len=bound)
+        _within(lse, l, tol_l)
+        _within(out, o, tol)

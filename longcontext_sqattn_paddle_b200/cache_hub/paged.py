@@ -43,6 +43,8 @@ class PageAllocator:
 class PagedKVCache:
     """``flash_attn_cache``'s methods over pages.
 
+    A sequence of the batch begins with its prefill (or, after ``release``, with the next step's token) and takes part in every
+    decode step until ``end``: from then on steps leave it out, it holds no pages and its attention is zeros.
     ``kv_format``: "native" (the 16-bit type), "int8" or "int4" (one scale per token and KV head).  ``num_pages``: size of the pool
     (default: enough for every sequence to reach ``max_length``).  ``select_pages``: a decode step attends to so many pages per
     KV head, the first ``sink_pages``, the last ``recent_pages`` and the best scoring ones; None: to all of them."""
@@ -67,6 +69,9 @@ class PagedKVCache:
         self.valid_length = torch.zeros(batch_size, dtype=torch.int32, device=self.device)   # cached tokens
         self.valid_length_host = [0] * batch_size
         self.after = torch.zeros_like(self.valid_length)    # with the token of the step under way
+        self.at = torch.zeros_like(self.valid_length)       # where that token goes, -1 for a sequence that has ended
+        self.active = torch.ones_like(self.valid_length)    # 0: ended
+        self.active_host = [True] * batch_size
         self._zero = torch.zeros(1, dtype=torch.int32, device=self.device)
         self.context = 0
 
@@ -89,11 +94,18 @@ class PagedKVCache:
                 pool.k_bounds.copy_(b)
 
     def release(self, b: int) -> None:
-        """Sequence b ends: its pages are free for others."""
+        """The pages of sequence b are free for others, and the next step's token is its first again (``end``: there is none)."""
         self.allocator.release(b)
         self.block_table[b].fill_(-1)
         self.valid_length[b] = 0
         self.valid_length_host[b] = 0
+
+    def end(self, b: int) -> None:
+        """Sequence b has ended: its pages are free for others, and decode steps, captured ones too, leave it out until a prefill
+        begins another one in its place."""
+        self.release(b)
+        self.active[b] = 0
+        self.active_host[b] = False
 
     # ---- the layer loops' calls ----------------------------------------------------------------------------------
     def prefill_update_kv_cache(self, query_states, key_states, value_states, layer_idx, start_bdx):
@@ -107,6 +119,9 @@ class PagedKVCache:
             self.reserve(start_bdx, valid)
             self.valid_length[start_bdx] = valid
             self.valid_length_host[start_bdx] = valid
+            if not self.active_host[start_bdx]:
+                self.active[start_bdx] = 1
+                self.active_host[start_bdx] = True
         key, value = key_states[:, vs:], value_states[:, vs:]
         ops.paged_write(self.pools[layer_idx], key.to(self.dtype), value.to(self.dtype), self.block_table[start_bdx:start_bdx + 1], self._zero)
         if layer_idx == self.layer_num - 1 and start_bdx + bsz == self.batch_size:
@@ -120,17 +135,23 @@ class PagedKVCache:
         """The pages are on the GPU already."""
 
     def decode_update_kv_cache(self, key_states, value_states, layer_idx):
-        """Append one token per sequence; ``decode_attention`` of this layer sees it."""
+        """Append one token per sequence that has not ended; ``decode_attention`` of this layer sees it."""
         if layer_idx == 0:
             if not torch.cuda.is_current_stream_capturing():
                 for b, n in enumerate(self.valid_length_host):
-                    self.reserve(b, n + 1)
-            torch.add(self.valid_length, 1, out=self.after)
-        ops.paged_write(self.pools[layer_idx], key_states.to(self.dtype), value_states.to(self.dtype), self.block_table, self.valid_length)
+                    if self.active_host[b]:
+                        self.reserve(b, n + 1)
+            torch.add(self.valid_length, self.active, out=self.after)
+            torch.sub(self.after, 1, out=self.at)       # (an ended sequence has length 0)
+        ops.paged_write(self.pools[layer_idx], key_states.to(self.dtype), value_states.to(self.dtype), self.block_table, self.at)
         if layer_idx == self.layer_num - 1:
-            self.context += 1
-            self.valid_length += 1
-            self.valid_length_host = [n + 1 for n in self.valid_length_host]
+            self.valid_length.copy_(self.after)
+            self.count_step()
+
+    def count_step(self) -> None:
+        """The host's side of a step that has been appended."""
+        self.context += 1
+        self.valid_length_host = [n + int(a) for n, a in zip(self.valid_length_host, self.active_host)]
 
     def decode_attention(self, query, layer_idx, out_dtype=None):
         """query [B, 1, Hq, D] against the layer's pages, the step's own token among them -> [B, 1, Hq, D]."""

@@ -322,8 +322,11 @@ class RandomInitDecoder:
         self._g_ids.copy_(inputs_ids)
         self._graph.replay()
         kc = self.kv_cache
-        kc.context += 1
-        kc.valid_length_host = [x + 1 for x in kc.valid_length_host]
+        if self.paged_kv is not None:
+            kc.count_step()
+        else:
+            kc.context += 1
+            kc.valid_length_host = [x + 1 for x in kc.valid_length_host]
         return self._g_logits
 
     # ---- generation (model_hub/LLM.py:160-235, model_hub/qwen.py:269-290) ------------------------------

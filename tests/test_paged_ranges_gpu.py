@@ -259,3 +259,53 @@ def test_decode_on_either_side_of_the_lines_between_its_forms(fmt, b, hkv, n):
         out, lse = _decode(q, pool, dtype, table, lens, max_kv_len=bound)
         _within(lse, l, tol_l)
         _within(out, o, tol)
+
+
+# ---- the cache -------------------------------------------------------------------------------------------------------
+def _cache(**kw):
+    from longcontext_sqattn_paddle_b200.cache_hub import PagedKVCache
+    return PagedKVCache(0, 1, 3, 256, 2, 4, 64, torch.float16, **{**dict(kv_format="int8", page_size=16), **kw})
+
+
+def _rows(b, n, seed):
+    return torch.randn(b, n, 2, 64, generator=_gen(seed)).half().cuda()
+
+
+def test_an_ended_sequence_takes_no_part_in_steps():
+    """It takes no pages, its length stays 0 and its attention is zeros, while the others go on; a prefill begins another in its
+    place."""
+    kc = _cache(num_pages=16)
+    for b, n in ((0, 40), (1, 100), (2, 48)):           # 3, 7 and 3 of the 16 pages
+        kc.prefill_update_kv_cache(None, _rows(1, n, b), _rows(1, n, 10 + b), 0, b)
+    kc.end(1)
+    q = torch.randn(3, 1, 4, 64, generator=_gen(281)).half().cuda()
+    for t in range(70):                                 # the two others need 13 pages in the end
+        kc.decode_update_kv_cache(_rows(3, 1, 100 + t), _rows(3, 1, 200 + t), 0)
+        out = kc.decode_attention(q, 0)
+        assert (out[1] == 0).all() and (out[0] != 0).any() and (out[2] != 0).any()
+    assert kc.valid_length.tolist() == kc.valid_length_host == [110, 0, 118]
+    assert kc.allocator.pages[1] == [] and (kc.block_table[1] == -1).all() and len(kc.allocator.free) == 16 - 7 - 8
+    key = kc.read(0, 0, 40, 70)[0][0].float()
+    want = torch.cat([_rows(3, 1, 100 + t)[0] for t in range(70)]).float()
+    assert ((key - want).abs() <= want.abs().amax(-1, keepdim=True) / 100).all()
+    kc.prefill_update_kv_cache(None, _rows(1, 10, 5), _rows(1, 10, 6), 0, 1)
+    kc.decode_update_kv_cache(_rows(3, 1, 7), _rows(3, 1, 8), 0)
+    assert kc.valid_length.tolist() == kc.valid_length_host == [111, 11, 119]
+    assert (kc.decode_attention(q, 0)[1] != 0).any()
+
+
+def test_a_sequence_ends_between_captured_steps():
+    from test_paged_cache_gpu import _model, _prefill
+    m = _model(dict(kv_format="int8", page_size=16))
+    ids = torch.randint(0, 2048, (2, 90), generator=_gen(282)).cuda()
+    _prefill(m, ids, 40)
+    m.capture_decode_step(2)
+    tok = torch.full((2, 1), 5, device="cuda")
+    m.decode_forward_graph(tok)
+    m.kv_cache.end(0)
+    for _ in range(3):
+        logits = m.decode_forward_graph(tok)
+    assert logits.isfinite().all()
+    kc = m.kv_cache
+    assert kc.valid_length.tolist() == kc.valid_length_host == [0, 94] and kc.context == 94
+    assert kc.allocator.pages[0] == []

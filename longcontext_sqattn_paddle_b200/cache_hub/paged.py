@@ -77,11 +77,18 @@ class PagedKVCache:
 
     # ---- pages ---------------------------------------------------------------------------------------------------
     def reserve(self, b: int, tokens: int) -> None:
-        """Room for ``tokens`` tokens of sequence b (a captured decode step needs it beforehand for all it will append)."""
+        """Room for ``tokens`` tokens of sequence b."""
         have = len(self.allocator.pages[b])
         new = self.allocator.reserve(b, tokens)
         if new:
             self.block_table[b, have:have + len(new)] = torch.tensor(new, dtype=torch.int32).to(self.device)
+
+    def reserve_step(self) -> None:
+        """Room for the next token of every sequence that has not ended; before the replay of a captured step, which reads the table
+        on the device but takes no pages of its own."""
+        for b, n in enumerate(self.valid_length_host):
+            if self.active_host[b]:
+                self.reserve(b, n + 1)
 
     def bounds(self):
         """Copies of the pages' key bounds, for ``restore_bounds`` after steps that are taken back: a row that is written again
@@ -138,9 +145,7 @@ class PagedKVCache:
         """Append one token per sequence that has not ended; ``decode_attention`` of this layer sees it."""
         if layer_idx == 0:
             if not torch.cuda.is_current_stream_capturing():
-                for b, n in enumerate(self.valid_length_host):
-                    if self.active_host[b]:
-                        self.reserve(b, n + 1)
+                self.reserve_step()
             torch.add(self.valid_length, self.active, out=self.after)
             torch.sub(self.after, 1, out=self.at)       # (an ended sequence has length 0)
         ops.paged_write(self.pools[layer_idx], key_states.to(self.dtype), value_states.to(self.dtype), self.block_table, self.at)

@@ -284,9 +284,6 @@ class RandomInitDecoder:
         if kc is None or kc.valid_length is None or not kc.allocated:
             raise RuntimeError("capture_decode_step needs a prefilled, GPU-resident cache")
         dev = self.device
-        if self.paged_kv is not None:
-            for b in range(batch_size):   # a replayed step takes no pages of its own
-                kc.reserve(b, kc.max_length)
         self._g_ids = torch.zeros(batch_size, 1, dtype=torch.int64, device=dev)
         self._g_pos = torch.full((1,), kc.context, dtype=torch.int64, device=dev)
         self._g_lens = torch.zeros(batch_size, dtype=torch.int32, device=dev)
@@ -319,9 +316,11 @@ class RandomInitDecoder:
 
     def decode_forward_graph(self, inputs_ids):
         """``decode_forward`` through the captured graph; returns a view of the graph's logits buffer."""
+        kc = self.kv_cache
+        if self.paged_kv is not None:
+            kc.reserve_step()
         self._g_ids.copy_(inputs_ids)
         self._graph.replay()
-        kc = self.kv_cache
         if self.paged_kv is not None:
             kc.count_step()
         else:

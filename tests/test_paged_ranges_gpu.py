@@ -309,3 +309,35 @@ def test_a_sequence_ends_between_captured_steps():
     kc = m.kv_cache
     assert kc.valid_length.tolist() == kc.valid_length_host == [0, 94] and kc.context == 94
     assert kc.allocator.pages[0] == []
+
+
+def test_captured_steps_take_pages_as_they_go():
+    """A pool smaller than all sequences at their longest; a sequence that is prefilled anew after the capture; a pool that runs out
+    refuses the step before it has run."""
+    from test_paged_cache_gpu import _model, _prefill
+    options = dict(kv_format="int8", page_size=16, num_pages=12)
+    ids = torch.randint(0, 2048, (2, 60), generator=_gen(291)).cuda()
+    eager, graphed = _model(options), _model(options)
+    _prefill(eager, ids, 200), _prefill(graphed, ids, 200)      # 17 pages a sequence at the longest
+    graphed.capture_decode_step(2)
+    assert len(graphed.kv_cache.allocator.free) == 4
+    tok = torch.full((2, 1), 5, device="cuda")
+    for t in range(36):                                         # to 96 tokens, all twelve pages
+        a, b = eager.decode_forward(tok), graphed.decode_forward_graph(tok)
+        assert (a - b).abs().max().item() < 0.03 * a.abs().max().item()
+        tok = torch.full_like(tok, 7 + 3 * t)
+    assert graphed.kv_cache.allocator.free == [] and graphed.kv_cache.valid_length.tolist() == [96, 96]
+    with pytest.raises(RuntimeError, match="exhausted"):
+        graphed.decode_forward_graph(tok)
+    kc = graphed.kv_cache
+    assert kc.valid_length.tolist() == kc.valid_length_host == [96, 96]
+    kc.end(0)
+    g = _gen(292)
+    k, v = (torch.randn(1, 14, 2, 128, generator=g).bfloat16().cuda() for _ in range(2))
+    for layer in range(2):
+        kc.prefill_update_kv_cache(None, k, v, layer, 0)
+    for _ in range(5):                                          # the third step's token needs a second page
+        graphed.decode_forward_graph(tok)
+    assert kc.valid_length.tolist() == kc.valid_length_host == [19, 101] and len(kc.allocator.pages[0]) == 2
+    key = kc.read(1, 0)[0][0].float()
+    assert ((key[:14] - k[0].float()).abs() <= k[0].float().abs().amax(-1, keepdim=True) / 100).all() and (key[14:].abs().amax(-1) > 0).all()

@@ -165,8 +165,8 @@ class PagedKVCache:
             pages = ops.paged_select(query, pool, self.block_table, self.after, self.select_pages, sink_pages=self.sink_pages,
                                      recent_pages=self.recent_pages)
             return ops.paged_decode(query, pool, self.block_table, self.after, pages=pages, out_dtype=out_dtype)
-        # the lengths that a captured launch will see are not known here
-        bound = 0 if torch.cuda.is_current_stream_capturing() else max(self.valid_length_host) + 1
+        # the lengths that a captured launch will see are not known here; elsewhere a bound that changes now and then, not with every token
+        bound = 0 if torch.cuda.is_current_stream_capturing() else -(-(max(self.valid_length_host) + 1) // 512) * 512
         return ops.paged_decode(query, pool, self.block_table, self.after, max_kv_len=bound, out_dtype=out_dtype)
 
     def read(self, layer_idx, b: int, start: int = 0, num_tokens: Optional[int] = None):

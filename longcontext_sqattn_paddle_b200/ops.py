@@ -608,11 +608,14 @@ def paged_read(pool: PagedPool, block_table, starts, num_rows: int, ends=None, o
 
 
 def _paged_scratch(pool: PagedPool, a, sizes, query):
-    """A workspace for the call; its size follows from ``sizes`` alone and is asked for once."""
+    """A workspace for the call; its size follows from ``sizes`` alone and is asked for once (a table or batch that changes with
+    every call does not make the list of known sizes grow for good)."""
     need = pool._scratch.get(sizes)
     if need is None:
         need = query(C.byref(a))
         if need:
+            if len(pool._scratch) >= 64:
+                pool._scratch.clear()
             pool._scratch[sizes] = need
     if need:
         ws = _paged_empty(pool, (need,), (1,), torch.uint8)   # the caching allocator's blocks are 512-byte aligned
@@ -644,10 +647,11 @@ def paged_decode(q, pool: PagedPool, block_table, kv_lens, *, pages=None, max_kv
     out_code = _dt(out_dtype)
     out = _paged_empty(pool, (b, 1, hq, d) if layout == "NHD" else (b, hq, 1, d), (hq * d, hq * d, d, 1) if layout == "NHD" else (hq * d, d, d, 1), out_dtype)
     lse = _paged_empty(pool, (b, hq, 1), (hq, 1, 1), torch.float32) if return_lse else None
+    max_kv_len = int(max_kv_len)
     if b:
         a = L.PagedDecodeArgs.from_buffer(bytearray(_PAGED_DECODE_ARGS.pack(
             pool._address, *qd, out.data_ptr(), hq * d, d, hq * d, 0 if lse is None else lse.data_ptr(), table, stride, lens, list_at,
-            b, hq, max_pages, listed, out_code, int(max_kv_len), float(sm_scale), 0, 0)))
+            b, hq, max_pages, listed, out_code, max_kv_len, float(sm_scale), 0, 0)))
         ws = _paged_scratch(pool, a, ("decode", b, hq, max_pages, listed, max_kv_len), L.lib.sqattn_paged_decode_workspace_bytes)
         _on_device(pool, L.lib.sqattn_paged_decode, C.byref(a))
         del ws

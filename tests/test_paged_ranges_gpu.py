@@ -341,3 +341,20 @@ def test_captured_steps_take_pages_as_they_go():
     assert kc.valid_length.tolist() == kc.valid_length_host == [19, 101] and len(kc.allocator.pages[0]) == 2
     key = kc.read(1, 0)[0][0].float()
     assert ((key[:14] - k[0].float()).abs() <= k[0].float().abs().amax(-1, keepdim=True) / 100).all() and (key[14:].abs().amax(-1) > 0).all()
+
+
+def test_known_workspace_sizes_do_not_pile_up():
+    """Neither over the steps of a cache nor with a bound or a table that changes in every call."""
+    ops = _ops()
+    kc = _cache(num_pages=48, kv_format="native")
+    for b in range(3):
+        kc.prefill_update_kv_cache(None, _rows(1, 20, b), _rows(1, 20, b), 0, b)
+    q = torch.randn(3, 1, 4, 64, generator=_gen(301)).half().cuda()
+    for t in range(100):
+        kc.decode_update_kv_cache(_rows(3, 1, 0), _rows(3, 1, 1), 0)
+        kc.decode_attention(q, 0)
+    assert len(kc.pools[0]._scratch) == 1
+    want = kc.decode_attention(q, 0)
+    for bound in range(121, 400):
+        assert torch.equal(ops.paged_decode(q, kc.pools[0], kc.block_table, kc.after, max_kv_len=bound), want)
+    assert len(kc.pools[0]._scratch) <= 64

@@ -497,7 +497,7 @@ class PagedPool:
 
 # A CUDA tensor on the current device without the argument parser of torch.empty: 0.9 us against 2.4, of calls whose kernels take 3 to
 # 10.  (Inductor's allocation entry; torch.empty where a torch build has none.)
-_empty_strided = getattr(torch._C._dynamo.guards, "_empty_strided_cuda", None)
+_empty_strided = getattr(getattr(getattr(torch._C, "_dynamo", None), "guards", None), "_empty_strided_cuda", None)
 
 
 def _paged_empty(pool: "PagedPool", shape, strides, dtype):

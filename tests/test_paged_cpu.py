@@ -122,3 +122,14 @@ def test_selection_budgets_that_are_refused():
     from longcontext_sqattn_paddle_b200.cache_hub import PagedKVCache
     with pytest.raises(ValueError):
         PagedKVCache(0, 1, 1, 64, 2, 4, 64, torch.float16, select_pages=2, sink_pages=1, recent_pages=2, device="cpu")
+
+
+def test_import_without_the_inductor_allocator():
+    """A torch build without that private module has the public allocator."""
+    import os
+    import subprocess
+    import sys
+    code = ("import torch\ndel torch._C._dynamo.guards\nfrom longcontext_sqattn_paddle_b200 import ops\n"
+            "assert ops._empty_strided is None\n")
+    done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+    assert done.returncode == 0, done.stderr

@@ -358,3 +358,91 @@ def test_known_workspace_sizes_do_not_pile_up():
     for bound in range(121, 400):
         assert torch.equal(ops.paged_decode(q, kc.pools[0], kc.block_table, kc.after, max_kv_len=bound), want)
     assert len(kc.pools[0]._scratch) <= 64
+
+
+def _stretch(fmt, dtype, hkv, group, lens, ps, seed, d=128, distinct=None, pages=None):
+    """Against the definition, over a pool of ``distinct`` pages that sequences share."""
+    per = (max(lens) + ps - 1) // ps
+    distinct = distinct or per * len(lens)
+    pool = _cuda(_full(fmt, dtype, distinct, hkv, ps, d, seed))
+    table = torch.randint(0, distinct, (len(lens), per), generator=_gen(seed + 1), dtype=torch.int32).cuda()
+    q = torch.randn(len(lens), hkv * group, d, generator=_gen(seed + 2)).to(dtype).cuda()
+    o, l, tol, tol_l = _bounds(q, pool, fmt, table, lens, dtype, pages=pages, one_part=fmt != "native" and dtype == torch.bfloat16)
+    out, lse = _decode(q, pool, dtype, table, lens, **({} if pages is None else {"pages": _i32(pages)}))
+    empty = l == -float("inf")                               # no keys: no tokens, or none of the listed pages is held
+    assert (out[empty] == 0).all() and (lse[empty] == -float("inf")).all()
+    _within(lse[~empty], l[~empty], tol_l[~empty])
+    _within(out, o, tol)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("hkv,group,ps,lens", [
+    (1, 7, 64, [20001]),                                     # all CTAs on one segment, their parts joined by rows
+    (1, 16, 128, [12000]),
+    (4, 12, 32, [9001, 8200]),
+    (3, 8, 16, [30000, 1, 0, 8193, 77]),                     # the same beside segments that lie in one warp
+])
+def test_stretches_of_few_long_sequences(dtype, fmt, hkv, group, ps, lens):
+    _stretch(fmt, dtype, hkv, group, lens, ps, 311)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("hkv,group,ps,lens", [
+    (8, 4, 32, [3000, 10, 0, 700, 64, 1500, 33, 2049] * 3),  # 192 segments: several tiles a warp, whole ones and cut ones, joined by cuts
+    (8, 16, 64, [900, 2500, 1, 4000] * 5),
+    (1, 9, 16, [1200 + 37 * i for i in range(160)]),
+])
+def test_stretches_of_many_sequences(dtype, fmt, hkv, group, ps, lens):
+    _stretch(fmt, dtype, hkv, group, lens, ps, 321, distinct=300)
+
+
+@pytest.mark.parametrize("fmt,n", [("native", 170001), ("int8", 170001), ("int4", 500003)])
+def test_stretches_of_more_tiles_than_a_warp_looks_up_at_once(fmt, n):
+    """More than 32 tiles a warp."""
+    _stretch(fmt, torch.bfloat16, 8, 4, [n], 128, 331, distinct=40)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("group", [5, 16])
+def test_stretches_over_listed_pages(fmt, group):
+    """Lists of 20 pages for 24 segments, holes and pages past the end among them."""
+    g = _gen(341)
+    lens = [4000, 90, 2222]
+    pages = [[torch.where(torch.rand(20, generator=g) < 0.2, -1, torch.randperm(70, generator=g)[:20]).tolist() for _ in range(8)] for _ in lens]
+    _stretch(fmt, torch.float16, 8, group, lens, 64, 342, pages=pages)
+
+
+# ---- selection over many pages ---------------------------------------------------------------------------------------
+@pytest.mark.parametrize("held,budget,sink,recent,distinct", [
+    (16384, 100, 1, 1, 16384),                               # as many as stay in registers
+    (16385, 100, 1, 1, 16385),                               # one more: the keys are read again in every round
+    (40000, 3000, 4, 7, 40000),
+    (40000, 17000, 1, 2, 3),                                 # pages of three kinds: the budget ends among equal ones, past the first 16384
+    (40000, 9, 4, 5, 40000),                                 # nothing left to choose
+    (131072, 1, 0, 0, 1),                                    # the most pages there may be, all alike
+    (131072, 70000, 0, 1, 90000),
+])
+def test_select_over_many_pages(held, budget, sink, recent, distinct):
+    ops = _ops()
+    dtype, d, hkv, group = torch.bfloat16, 64, 2, 3
+    g = _gen(351)
+    bounds = torch.randn(distinct, hkv, 2, d, generator=g).to(dtype).sort(dim=2).values
+    pool = _empty("int8", dtype, 1, hkv, 16, d)
+    pool = {n: t.expand(distinct, *t.shape[1:]).contiguous() for n, t in pool.items()}
+    pool["k_bounds"] = bounds
+    table = torch.cat((torch.randperm(distinct, generator=g), torch.randint(0, distinct, (held - distinct,), generator=g))).to(torch.int32)[None]
+    if held > 20000 and distinct > 3:
+        table[0, 16390], table[0, 5] = -1, distinct          # pages that are not there
+    q = torch.randn(1, hkv * group, d, generator=g).to(dtype)
+    got = ops.paged_select(q[:, None].cuda(), _handle(_cuda(pool), dtype), table.cuda(), _i32([held * 16 - 3]), budget, sink_pages=sink, recent_pages=recent)
+    u = q.view(hkv, group, d).double().sum(1)
+    at = torch.arange(held)
+    there = (table[0] >= 0) & (table[0] < distinct)
+    for h in range(hkv):
+        low, high = bounds[table[0].long().clamp(0, distinct - 1), h].double().unbind(1)
+        score = torch.where(there, torch.maximum(u[h] * low, u[h] * high).sum(-1), -float("inf"))
+        score[(at < sink) | (at >= held - recent)] = float("inf")
+        best = torch.sort(score, descending=True, stable=True).indices[:budget].sort().values
+        assert got[0, h].tolist() == best.tolist()

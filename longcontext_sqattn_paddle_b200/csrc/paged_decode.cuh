@@ -513,7 +513,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         // a power of two brings the largest to [2^22, 2^23), sums come back in units of 2^8; 4-bit codes arrive 16 times as large
         const uint32_t e = max(__float_as_uint(top) >> 23, 27u);
         const float up = __uint_as_float((276u - e) << 23);
-        const float down = e == 255u ? __int_as_float(0x7fc00000) : p.scale_log2 * __uint_as_float((e - (FMT == kKvInt4 ? 18u : 14u)) << 23);
+        const float down = e == 255u ? __int_as_float(0x7fc00000) : p.scale_log2 * __uint_as_float((e - (FMT == kKvInt4 ? 6u : 2u)) << 23);   // 2^12 of the key scales' too
 #pragma unroll
         for (int j = 0; j < D / 32; ++j)
 #pragma unroll
@@ -630,7 +630,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
           for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
             for (int hi = 0; hi < 2; ++hi) {
-              const float ks = sc[mt * 16 + hi * 8 + key_row];
+              const float ks = sc[mt * 16 + hi * 8 + key_row] * (1.0f / 4096.0f);   // sums of up to 2^30: keys near the type's largest stay in range
               vs[mt][hi] = sc[TILE + mt * 16 + hi * 8 + key_row];
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt) { s[nt][mt][2 * hi] *= ks; s[nt][mt][2 * hi + 1] *= ks; }

@@ -446,3 +446,27 @@ def test_select_over_many_pages(held, budget, sink, recent, distinct):
         score[(at < sink) | (at >= held - recent)] = float("inf")
         best = torch.sort(score, descending=True, stable=True).indices[:budget].sort().values
         assert got[0, h].tolist() == best.tolist()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("group,lens", [(8, [500]), (3, [20, 9000])])
+def test_decode_of_keys_near_the_types_range(fmt, group, lens):
+    """bf16 keys of up to 2^119, scores of ordinary size."""
+    dtype, d, hkv, ps = torch.bfloat16, 128, 1, 64
+    per = (max(lens) + ps - 1) // ps
+    g = _gen(361)
+    table = torch.arange(per * len(lens), dtype=torch.int32).view(len(lens), per)
+    got = _cuda(_empty(fmt, dtype, per * len(lens), hkv, ps, d))
+    pool = _handle(got, dtype)
+    key, value = torch.randn(len(lens), max(lens), hkv, d, generator=g) * 2.0 ** 117, torch.randn(len(lens), max(lens), hkv, d, generator=g)
+    _ops().paged_write(pool, key.to(dtype).cuda(), value.to(dtype).cuda(), table.cuda(), _i32([0] * len(lens)))
+    q = (torch.randn(len(lens), group, d, generator=g) * 2.0 ** -97).to(dtype).cuda()
+    scale = 2.0 ** -23
+    out, lse = _decode(q, got, dtype, table, lens, sm_scale=scale)
+    o, l, spread, size, vmax = PO.attention(q, got, fmt, table.cuda(), lens, sm_scale=scale)
+    n = max(lens)
+    score = d * 2.0 ** -23 * size + (0.0 if fmt == "native" else 2.0 ** -23 * q.double().abs().amax(-1) * 2.0 ** 120 * d * scale)   # (as in _bounds)
+    tol = 2.0 ** -8 * o.abs() + (2.0 ** -11 + 2 * score + n * 2.0 ** -23)[..., None] * spread + n * 2.0 ** -39 * vmax[..., None]
+    assert 1 < size.max() < 100
+    _within(lse, l, (score + n * 2.0 ** -23) * 1.4427 + 2.0 ** -22 * (1 + l.abs()))
+    _within(out, o, tol)

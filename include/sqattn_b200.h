@@ -419,8 +419,8 @@ typedef struct {
 /* Write new rows: row i < counts[b] (counts NULL: i < num_rows) of k, v [B, Hkv, num_rows, D] becomes position
  * positions[b] + i of sequence b (positions, counts: device int32 [B]; a negative position writes nothing for that
  * sequence).  Position 0 of a page starts its bounds anew, later ones extend them (a row written again leaves them as wide as
- * they were).  Two sequences of one call must not
- * write into the same page.  Rows 16-byte aligned. */
+ * they were).  A call must not write into one page twice: two sequences must not share a page that they write to, and no table
+ * names a page twice where rows fall.  Rows 16-byte aligned. */
 int sqattn_paged_write(const sqattn_paged_pool* pool, const sqattn_tensor* k, const sqattn_tensor* v, int32_t batch,
                        int32_t num_rows, const int32_t* block_table, int64_t table_stride, int32_t max_pages,
                        const int32_t* positions, const int32_t* counts, sqattn_stream_t stream);
@@ -449,7 +449,8 @@ typedef struct {
 
 /* o = softmax(sm_scale * q k^T) v over the first kv_lens[b] cached tokens (or those of them in the listed pages); at most
  * 16 query heads per KV head and 1024 sequences.  Softmax statistics and sums in fp32.  Codes enter the products exactly; with
- * them a query channel is off by at most 2^-23 of its head's largest.  Infinities and NaN go where the formula takes them: an
+ * them a query channel is off by at most 2^-23 of its head's largest, and a weight by 2^-11 where outputs are bf16 (f16 outputs,
+ * and native pages: 2^-15 at most).  Infinities and NaN go where the formula takes them: an
  * infinite value of a key whose weight fp32 can hold makes its channel infinite (NaN beside one of the other sign), and a
  * sequence whose scores are all -inf, or of which one is +inf or NaN, gets NaN (its LSE is -inf or NaN). */
 size_t sqattn_paged_decode_workspace_bytes(const sqattn_paged_decode_args* args);

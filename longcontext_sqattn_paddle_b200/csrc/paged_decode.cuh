@@ -15,13 +15,14 @@
 //
 // Arithmetic.  S^T = K Q^T and O^T = V^T P^T on mma.sync m16n8k16 with the keys (channels) as rows and the query heads as
 // the 8 columns: with at most 8 heads to a group no product is padding but the unused heads' columns.  The products do not
-// bound the kernel (a key takes 0.25 KFLOP a head for 128-512 bytes), so the tcgen05 path, which would need 64 or 128
+// bound the kernel (at 128 channels a key takes 0.5 KFLOP a head for 128-512 bytes), so the tcgen05 path, which would need 64 or 128
 // rows of queries, has nothing to give here.
 //   codes, scores: integer products m16n8k32 of the keys' bytes as they lie (4-bit codes as the high halves of bytes: a mask) with
 //     q as 24-bit integers, a power of two per head high, in a signed high and two unsigned lower bytes: sums are exact, and q is
 //     off by at most 2^-23 of the head's largest, half a step of fp32.  Two bytes (2^-15) are not enough beside a head's large
-//     channels: with one of 64 times the others scores were off by 1e-3.  The third product costs 512K int4 tokens 67.0 -> 71.4 us,
-//     64 ragged int4 sequences 76.4 -> 78.8, int8 0.5 %; leaving it out for heads without large channels gains 0.5 us of that.
+//     channels: with one of 64 times the others scores were off by 1e-3.  The third product costs 512K int4 tokens 66.6 -> 70.8 us,
+//     64 ragged int4 sequences 78.0 -> 80.4, 16 ragged int8 ones 152 -> 157; leaving it out for heads without large channels gains
+//     0.5 us of that, adding `low` up in integers nothing.
 //   codes, output: codes become f16 exactly by exponent tricks; a value's scale multiplies its weight p in fp32, and the product
 //     is rounded to f16 relative to the largest value scale so far (as a power of two), 2^14 high.  For bf16 outputs that
 //     rounding (2^-11) vanishes beside theirs (2^-8); for f16 outputs, which have the same, the weight is split as below.  The
@@ -78,7 +79,8 @@ struct PagedDecodeCfg {
   static constexpr int kRow = kv_row_bytes<FMT>(D);
   // Measured (us; 1M native | 16 ragged int8 | 512K int4, 28/4 and 32/8 heads): native 8 warps of one tile in flight 319, 4 of two
   // 321, of three 338-351; int8 8 of two 131, 10 137, 12 147, 6 149; int4 12 warps of two 64-key tiles 68, of two 32-key tiles 75,
-  // 16 of two 32-key tiles 84, 8 86.  More than about 130 KB in flight an SM is slower, whatever holds it.
+  // 16 of two 32-key tiles 84, 8 86.  More than about 130 KB in flight an SM is slower, whatever holds it.  (Codes: with queries of
+  // two bytes.  With three, 512K int4 tokens take 12 warps 70.8, 11 75.5, 10 79.2.)
   static constexpr int kTile = FMT == kKvInt4 ? 64 : 32;                 // keys of a tile
   static constexpr int kWarps = FMT == kKvInt4 && NT == 1 ? 12 : 8;
   static constexpr int kStages = FMT == kKvNative && D == 128 ? 1 : 2;   // tiles a warp has in flight

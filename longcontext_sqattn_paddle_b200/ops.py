@@ -565,7 +565,7 @@ def _paged_query(pool: PagedPool, q, layout: str):
 def paged_write(pool: PagedPool, key, value, block_table, positions, counts=None) -> None:
     """sqattn_paged_write: quantise new rows into pages.  key / value [B, N, Hkv, D] (any strides) become positions
     ``positions[b] ...`` of the sequences whose pages ``block_table`` [B, max_pages] names; of each only the first
-    ``counts[b]`` rows (int32 [B], None: all N).  Two sequences of one call must not write into the same page."""
+    ``counts[b]`` rows (int32 [B], None: all N).  A call must not write into one page twice, for two sequences or for one."""
     if key.shape != value.shape:
         raise ValueError(f"key and value must have one shape, got {tuple(key.shape)} and {tuple(value.shape)}")
     key, kd = _paged_rows(pool, key, "key")

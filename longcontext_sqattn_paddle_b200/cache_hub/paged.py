@@ -116,7 +116,7 @@ class PagedKVCache:
 
     # ---- the layer loops' calls ----------------------------------------------------------------------------------
     def prefill_update_kv_cache(self, query_states, key_states, value_states, layer_idx, start_bdx):
-        """Write the valid part of one sequence's K/V into its pages, on the current stream."""
+        """Write the valid part of one sequence's K/V into its pages from the first on, on the current stream."""
         bsz, seq_len, _, _ = key_states.shape
         assert bsz == 1, "Multi-batch prefilling only support prefill single batch one by one."
         assert seq_len <= self.max_length, f"Prefilling sequence length {seq_len} exceeds max length {self.max_length}."
@@ -170,7 +170,8 @@ class PagedKVCache:
         return ops.paged_decode(query, pool, self.block_table, self.after, max_kv_len=bound, out_dtype=out_dtype)
 
     def read(self, layer_idx, b: int, start: int = 0, num_tokens: Optional[int] = None):
-        """Keys and values [1, tokens, Hkv, D] of one sequence as they are cached (for a prefill that continues it)."""
+        """Keys and values [1, tokens, Hkv, D] of one sequence as they are cached, for a caller whose own prefill continues it (the rows
+        of that go behind them by ``reserve`` and ``ops.paged_write``; ``prefill_update_kv_cache`` begins a sequence anew)."""
         n = self.valid_length_host[b] - start if num_tokens is None else num_tokens
         starts = torch.full((1,), start, dtype=torch.int32, device=self.device)
         return ops.paged_read(self.pools[layer_idx], self.block_table[b:b + 1], starts, n, self.valid_length[b:b + 1])
